@@ -574,6 +574,8 @@ PKM_API int pkm_batchnorm_bwd(const void* dy, const void* x, int x_dtype, int64_
  *   lse [B, Hq, Tq] fp32 receives the log of the softmax's sum (-inf for a
  *   row with nothing visible) and out_lo, in out's layout, what out's rounding
  *   left, rounded; both NULL when no backward pass follows.
+ * Inside [starts, ends) non-finite numbers act as in the formula: a visible
+ * score of NaN or +inf makes the row's output and lse NaN.
  * The forward pass needs pkm_attn_fwd_workspace() bytes (0 for most sizes: few
  * query tiles over many keys have their keys shared out and joined), the
  * backward pass pkm_attn_bwd_workspace(); 16-byte aligned, free for reuse once

@@ -8,7 +8,8 @@
 //   start <= j < end,  j <= p < end,  p >= start,
 //   and  window == 0  or  j > p - window  or  j < start + sinks,
 // [start, end) being the sequence's rows ([0, Tk) without the arrays).  A
-// query with nothing visible has output 0 and log-sum-exp -inf.
+// query with nothing visible (a row outside) has output 0 and log-sum-exp -inf;
+// one that sees a score of NaN or +inf, or only scores of -inf, has output NaN.
 #pragma once
 
 #include <math.h>

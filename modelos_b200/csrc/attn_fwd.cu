@@ -421,7 +421,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       if (!(ok = named_all(1 + i, ok))) break;
       const int id = 2 * w.pair + i;
       const int r0 = id / a.G * AT_T, h = w.hk * a.G + id % a.G, row = r0 + rl;
-      const bool some = row < a.Tq && pr >= 0 && pr < w.len && l > 0.f;
+      // which rows see something goes by position (a row sees itself at least),
+      // not by their sum, which a NaN or an infinite score makes NaN; a part of a
+      // split may have nothing for such a row
+      const bool some = row < a.Tq && pr >= 0 && pr < w.len && (a.splits == 1 || l != 0.f);
       if (a.lse && row < a.Tq)
         a.lse[((int64_t)w.ob * a.Hq + h) * a.Tq + row] = some ? (m + log2f(l)) * AT_LN2 : -INFINITY;
       const float inv = some ? 1.f / l : 0.f;
@@ -445,6 +448,7 @@ int attn_tmap(CUtensorMap* m, const void* p, int dtype, const Strides3& s, int64
 }
 
 // The parts of a split joined in their order: 16 lanes a row, as 128-bit pieces.
+// A part whose sum is NaN makes the row NaN (the maximum alone would pass over it).
 struct JoinArgs {
   const void* hi;  // [splits, B, Hq, Tq, D], and lo, lse
   const void* lo;
@@ -461,12 +465,20 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const JoinArgs j, FastDi
   const int d = (threadIdx.x & 15) * 8;
   const int64_t rows = (int64_t)a.B * a.Hq * a.Tq;
   float m = -INFINITY, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, j.lse[s * rows + r]);
-  if (m != -INFINITY) {
+  bool nan = false;
+  for (int s = 0; s < a.splits; ++s) {
+    const float e = j.lse[s * rows + r];
+    m = fmaxf(m, e);
+    nan |= isnan(e);
+  }
+  const Span sp = attn_span(a.starts, a.ends, (int)b, a.Tk);
+  const int p = (int)t + a.Tk - a.Tq;
+  const bool real = p >= sp.start && p < sp.end;
+  if (real) {
     for (int s = 0; s < a.splits; ++s) {
-      const float w = expf(j.lse[s * rows + r] - m);
+      const float w = expf(j.lse[s * rows + r] - m);  // (NaN where every score is -inf: 0 / 0)
       sum += w;
-      if (d < a.D && w > 0.f) {
+      if (d < a.D) {
         float hi[8], lo[8];
         const int64_t at = (s * rows + r) * a.D + d;
         VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(j.hi) + at), hi);
@@ -492,7 +504,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const JoinArgs j, FastDi
     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     if (a.out_lo) *reinterpret_cast<uint4*>(static_cast<T*>(a.out_lo) + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  if (a.lse && d == 0) a.lse[r] = m == -INFINITY ? m : m + logf(sum);
+  if (a.lse && d == 0) a.lse[r] = !real ? -INFINITY : nan ? NAN : m == -INFINITY ? m : m + logf(sum);
 }
 
 bool attn_few_rows(int64_t B, int64_t Hk, int64_t G, int64_t Tq) {

@@ -1,0 +1,131 @@
+"""NaN and infinities in rows that are seen, on the GPU kernels: the output, the
+softmax's logarithm and the gradients are what the definition gives, and never
+a finite number in place of a NaN."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import attnref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF = torch.bfloat16, torch.float16
+NAN, INF = float("nan"), float("inf")
+
+
+def make(B, Hq, Hk, Tq, Tk, D, dtype, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def t(H, T):
+        return torch.randn(B, T, H, D, generator=g, device=DEV).to(dtype).transpose(1, 2)
+
+    return t(Hq, Tq), t(Hk, Tk), t(Hk, Tk), t(Hq, Tq)
+
+
+def expected(q, k, v, window, sinks, scale, starts=None, lengths=None):
+    """``(out, lse, tol)`` in 64 bits.  A score of -inf is a probability of 0, one
+    of +inf or NaN makes the row NaN, as a row is whose scores are all -inf."""
+    Hq, Tq = q.shape[1:3]
+    see = attnref.visible(q.shape[0], Tq, k.shape[2], window, sinks, starts, None, lengths, DEV)
+    ks, vs = attnref.spread(k.double(), Hq), attnref.spread(v.double(), Hq)
+    s = torch.stack([q[b].double() @ ks[b].transpose(-1, -2) for b in range(len(q))]) * scale
+    s = s.masked_fill(~see, -INF)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - lse[..., None])
+    none = ~see.any(-1, keepdim=True)
+    p = torch.where(none, torch.zeros_like(p), p)
+    # hidden keys take no part, whatever they hold
+    out = torch.where(see[..., None], p[..., None] * vs[:, :, None], torch.zeros((), dtype=p.dtype, device=DEV)).sum(-2) \
+        if vs.isnan().any() else p @ vs
+    # as attnref.reference has it; the scores' size from the finite keys alone
+    u = torch.finfo(q.dtype).eps / 2
+    least = torch.finfo(q.dtype).smallest_normal * u
+    size = (torch.nan_to_num(q.double(), 0, 0, 0).abs() @ torch.nan_to_num(ks, 0, 0, 0).abs().transpose(-1, -2)) * scale
+    E = attnref.EXP + 2 * (q.shape[-1] + 4) * attnref.F32 * (size * see).amax().item()
+    n = see.sum(-1).amax().item()
+    va = torch.nan_to_num(vs, 0, 0, 0).abs()
+    a = torch.nan_to_num(p, 0, 0, 0) @ va
+    tol = u * torch.nan_to_num(out, 0, 0, 0).abs() + (u + 2 * E + (n + 8) * attnref.F32) * a * 1.01 + least * (
+        see.double() @ va)
+    return out, lse, tol
+
+
+def compare(got, want, tol, what):
+    bad = want.isnan()
+    assert bad.any(), what
+    assert torch.equal(got.isnan(), bad), f"{what}: {int((got.isnan() != bad).sum())} of {bad.numel()} are NaN wrongly"
+    attnref.within(got[~bad], want[~bad], tol[~bad], what)  # (none where every row sees the bad key)
+
+
+# tiles of 128 rows; keys shared by several blocks
+SHAPES = [(2, 4, 2, 300, 300), (1, 2, 1, 130, 1500)]
+
+
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64), (BF, 72)])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("what", ["k nan", "k inf", "q nan", "q inf"])
+def test_scores_that_are_not_finite(shape, dtype, D, what):
+    from modelos_b200.attention import window_attention
+    B, Hq, Hk, Tq, Tk = shape
+    q, k, v, _ = make(B, Hq, Hk, Tq, Tk, D, dtype, seed=Tk)
+    value = NAN if "nan" in what else INF
+    if what[0] == "k":
+        # one key early among the last queries' own, and (where they are not) one of the first block
+        k[0, 0, Tk - Tq + 1, 3] = value
+        k[-1, -1, 7 if Tk > Tq else Tk - 2, 3] = value
+    else:
+        q[0, 1, Tq // 2, 3] = value
+    for window, sinks in ((0, 0), (max(2, Tk // 4), 3)):
+        want, _, tol = expected(q, k, v, window, sinks, D ** -0.5)
+        got = window_attention(q, k, v, window=window, sinks=sinks)
+        compare(got, want, tol, (what, window))
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_value_that_is_not_finite(shape):
+    """In the rows that see it, and there in its channel alone."""
+    from modelos_b200.attention import window_attention
+    B, Hq, Hk, Tq, Tk = shape
+    q, k, v, _ = make(B, Hq, Hk, Tq, Tk, 64, BF, seed=Tk)
+    v[0, 0, 7 if Tk > Tq else 0, 3] = NAN  # all rows see it
+    want, _, tol = expected(q, k, v, 0, 0, 0.125)
+    compare(window_attention(q, k, v), want, tol, "v")
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_rows_whose_scores_are_all_minus_infinity(shape):
+    """0 / 0, not the 0 of a row that sees nothing; rows outside the sequence
+    stay 0, whatever they hold."""
+    from modelos_b200.attention import window_attention
+    B, Hq, Hk, Tq, Tk = shape
+    q, k, v, _ = make(B, Hq, Hk, Tq, Tk, 64, BF, seed=Tk)
+    q[:, :, :, 5], k[:, :, :, 5] = 1.0, -INF
+    first = Tk - Tq + 1  # the first query is padding
+    starts = torch.full((B,), first, dtype=torch.int32, device=DEV)
+    out = window_attention(q, k, v, starts=starts)
+    assert (out[:, :, 0] == 0).all() and out[:, :, 1:].isnan().all()
+
+
+def test_log_of_the_softmax_sum_and_gradients():
+    """A bad query: its lse and dq are NaN, and dk and dv of the keys that it
+    sees; other queries' dq are right."""
+    from test_attention_gpu import attn_fwd
+
+    from modelos_b200.attention import window_attention
+    for Tq, Tk in ((260, 260), (130, 1500)):
+        q, k, v, dout = make(1, 2, 1, Tq, Tk, 64, BF, seed=Tk)
+        clean = q.clone()
+        q[0, 1, 2, 3] = NAN
+        _, lse = attn_fwd(q, k, v, 0.125, 0, 0, None, None)
+        assert lse[0, 1, 2].isnan() and int(lse.isnan().sum()) == 1
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        dq, dk, dv = torch.autograd.grad(window_attention(*leaves), leaves, dout)
+        r = attnref.reference(clean, k, v, 0, 0, 0.125, None, None, dout)
+        real = torch.ones(1, 2, Tq, dtype=torch.bool, device=DEV)
+        real[0, 1, 2] = False
+        assert dq[~real].isnan().all()
+        attnref.within(dq[real], r["dq"][real], r["dq_tol"][real], "dq")
+        seen = Tk - Tq + 3
+        assert dk[:, :, :seen].isnan().all() and dv[:, :, :seen].isnan().all()
+
