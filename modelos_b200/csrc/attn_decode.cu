@@ -500,12 +500,15 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
 #pragma unroll
     for (int w = 0; w < F::WARPS; ++w) mx = fmaxf(mx, warp_m[w * F::ROWS + r]);
     float sum = 0.f, ls = 0.f;
-    if (mx != -INFINITY) {
+    // (a warp without anything for the row has a sum of 0; one with a NaN score
+    // has a NaN, which the maximum does not show)
 #pragma unroll
-      for (int w = 0; w < F::WARPS; ++w) {
+    for (int w = 0; w < F::WARPS; ++w) {
+      const float lw = warp_l[w * F::ROWS + r];
+      if (lw != 0.f) {
         const float f = ex2(warp_m[w * F::ROWS + r] - mx);
         sum = fmaf(f, reinterpret_cast<const float*>(smem)[w * F::ROWS * DP + e], sum);
-        ls = fmaf(f, warp_l[w * F::ROWS + r], ls);
+        ls = fmaf(f, lw, ls);
       }
     }
     block_o[e] = sum;
@@ -532,30 +535,33 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
       x1 = block_o[r * DP + d + 1];
     } else {
       for (int s = 0; s < S; ++s) mx = fmaxf(mx, ld_cluster(mapa_shared(mm + r * 4, s)));
-      if (mx != -INFINITY)
-        for (int s = 0; s < S; ++s) {
-          const float f = ex2(ld_cluster(mapa_shared(mm + r * 4, s)) - mx);
-          const uint32_t p = mapa_shared(om + (r * DP + d) * 4, s);
-          sum = fmaf(f, ld_cluster(mapa_shared(lm + r * 4, s)), sum);
-          x0 = fmaf(f, ld_cluster(p), x0);
-          x1 = fmaf(f, ld_cluster(p + 4), x1);
-        }
+      for (int s = 0; s < S; ++s) {
+        const float ls = ld_cluster(mapa_shared(lm + r * 4, s));
+        if (ls == 0.f) continue;
+        const float f = ex2(ld_cluster(mapa_shared(mm + r * 4, s)) - mx);
+        const uint32_t p = mapa_shared(om + (r * DP + d) * 4, s);
+        sum = fmaf(f, ls, sum);
+        x0 = fmaf(f, ld_cluster(p), x0);
+        x1 = fmaf(f, ld_cluster(p + 4), x1);
+      }
     }
     const int qr = row0 + r, i = qr / a.G, h = hk * a.G + qr % a.G;
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    // a row of the sequence sees itself at least; its sum is 0 or NaN only if its scores are -inf or NaN
+    const bool real = base + i >= sp.start && base + i < sp.end;
+    const float inv = 1.f / sum;
     if (d < a.D) {
       const int64_t at = b * a.so.b + h * a.so.h + (int64_t)i * a.so.t + d;
-      const uint32_t hi = sum > 0.f ? pack2<T>(x0 * inv, x1 * inv) : 0u;
+      const uint32_t hi = real ? pack2<T>(x0 * inv, x1 * inv) : 0u;
       *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at) = hi;
       if (a.out_lo) {
         float f[2];
         unpack2<T>(hi, f);
         *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out_lo) + at) =
-            sum > 0.f ? pack2<T>(x0 * inv - f[0], x1 * inv - f[1]) : 0u;
+            real ? pack2<T>(x0 * inv - f[0], x1 * inv - f[1]) : 0u;
       }
     }
     if (a.lse && d == 0)
-      a.lse[((int64_t)b * a.Hq + h) * a.Tq + i] = sum > 0.f ? (mx + log2f(sum)) * AT_LN2 : -INFINITY;
+      a.lse[((int64_t)b * a.Hq + h) * a.Tq + i] = real ? (mx + log2f(sum)) * AT_LN2 : -INFINITY;
   }
   __syncwarp();
   if (a.splits > 1) cluster_sync_all();  // the others read this block's shared memory until here
