@@ -66,11 +66,13 @@ class PKMFeedForward(nn.Module):
         return out
 
 
-def attention_bounds(attention_mask: torch.Tensor, kv_length: int) -> torch.Tensor:
+def attention_bounds(attention_mask: torch.Tensor, kv_length: int, kv_offset: Optional[int] = None) -> torch.Tensor:
     """``[2, B]`` int32: the first real token of each row of a padding mask
-    ``[B, tokens]`` among its last ``kv_length`` columns, and one past the last
-    (equal where a row has none).  Real tokens must be consecutive."""
-    m = attention_mask[:, -kv_length:].to(torch.int32)
+    ``[B, tokens]`` among ``kv_length`` columns from ``kv_offset`` on (None: the
+    last), and one past the last (equal where a row has none).  Real tokens must
+    be consecutive."""
+    first = attention_mask.shape[1] - kv_length if kv_offset is None else kv_offset
+    m = attention_mask[:, max(first, 0):first + kv_length].to(torch.int32)
     first = m.argmax(1)
     last = m.shape[1] - m.flip(1).argmax(1)
     return torch.stack((first, torch.where(m.any(1), last, first))).to(torch.int32)
@@ -86,7 +88,13 @@ def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     if kv_offset and getattr(config, "attention_sinks", 0):
         raise ValueError("modelos_b200 attention: this cache has dropped the first tokens, which attention_sinks needs; "
                          "pass past_key_values=QuantizedCache(...) or a cache without sliding layers")
-    return None if attention_mask is None else attention_bounds(attention_mask, kv_length)
+    if attention_mask is None:
+        return None
+    # a column of the mask is a position; it may have columns for tokens to come
+    if attention_mask.shape[1] < kv_offset + kv_length:
+        raise ValueError(f"modelos_b200 attention: the mask has {attention_mask.shape[1]} columns for "
+                         f"{kv_offset + kv_length} tokens")
+    return attention_bounds(attention_mask, kv_length, kv_offset)
 
 
 def _attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None, **kwargs):

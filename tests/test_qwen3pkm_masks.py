@@ -1,0 +1,66 @@
+"""What transformers may hand to this package's attention as mask and
+arguments: right, or refused.  Without a GPU (stand-ins of the kernels)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import attnref
+import fake_native
+from modelos_b200 import qwen3pkm
+
+BF = torch.bfloat16
+MODEL = dict(vocab_size=96, hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4,
+             num_key_value_heads=2, head_dim=64, max_position_embeddings=512, tie_word_embeddings=False)
+WINDOW = dict(use_sliding_window=True, sliding_window=6, max_window_layers=1)  # the first layer sees everything
+
+
+@pytest.fixture(autouse=True)
+def stand_in(monkeypatch):
+    fake_native.install(monkeypatch)
+    attnref.install(monkeypatch)
+
+
+def model(kw, **extra):
+    return qwen3pkm.build_qwen3_pkm(dict(MODEL, **kw), dict(pkm_layers=[]), qwen3pkm.ATTENTION, dtype=BF, device="cpu",
+                                    **extra).eval()
+
+
+def ids(B, T):
+    return torch.randint(0, 96, (B, T), generator=torch.Generator().manual_seed(1))
+
+
+def rel(a, b):
+    return ((a.double() - b.double()).norm() / b.double().norm()).item()
+
+
+@pytest.mark.parametrize("kw", [{}, WINDOW])
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_mask_wider_than_the_keys_so_far(kw, quantized):
+    """A prompt in chunks, each called with the whole batch's mask: columns are
+    key positions."""
+    m = model(kw)
+    x, mask = ids(2, 12), torch.ones(2, 12, dtype=torch.long)
+    mask[1, :5] = 0
+    cache = qwen3pkm.QuantizedCache(m.config, 16) if quantized else None
+    with torch.no_grad():
+        want = m(x[:, :8], attention_mask=mask[:, :8], use_cache=False).logits
+        out = m(x[:, :8], attention_mask=mask, past_key_values=cache, use_cache=True)
+        real = mask[:, :8].bool()
+        assert torch.equal(out.logits[real], want[real])
+        out = m(x[:, 8:10], attention_mask=mask, past_key_values=out.past_key_values)
+        want = m(x[:, :10], attention_mask=mask[:, :10], use_cache=False).logits[:, 8:]
+    # one chunk or two, the same roundings up to their order; 4 bits lose 0.08 of keys and of values in two layers:
+    # 0.08 * 4 ** 0.5
+    assert rel(out.logits, want) < (0.16 if quantized else 2.0 ** -6)
+
+
+def test_a_mask_of_fewer_columns_than_keys_is_refused():
+    with pytest.raises(ValueError, match="columns"):
+        qwen3pkm._attention_mask(2, 1, 9, q_offset=8, attention_mask=torch.ones(2, 1, dtype=torch.long))
+
+
+def test_bounds_count_columns_from_the_first_key():
+    m = torch.tensor([[0, 0, 1, 1, 1, 1], [1, 1, 1, 1, 1, 0], [0, 0, 0, 0, 0, 1]])
+    assert qwen3pkm.attention_bounds(m, 4, 0).tolist() == [[2, 0, 0], [4, 4, 0]]
+    assert qwen3pkm.attention_bounds(m, 3, 1).tolist() == [[1, 0, 0], [3, 3, 0]]
