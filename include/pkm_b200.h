@@ -55,6 +55,7 @@ enum {
 #define PKM_DEVERR_INDEX 1u   /* an index outside [0, num_rows) was skipped */
 #define PKM_DEVERR_TIMEOUT 2u /* a bounded wait inside a kernel gave up */
 #define PKM_DEVERR_CAPACITY 4u /* a token's row was outside the key/value cache and was skipped */
+/* 8u: a padding mask with padding between real tokens (set by the Python side, never by a kernel) */
 
 /* Library version (major*10000 + minor*100 + patch). */
 PKM_API int pkm_version(void);

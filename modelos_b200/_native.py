@@ -223,11 +223,14 @@ def err_word(dev: torch.device) -> torch.Tensor:
 DEVERR_INDEX = 1
 DEVERR_TIMEOUT = 2
 DEVERR_CAPACITY = 4
+DEVERR_MASK = 8  # (no kernel sets it: qwen3pkm.attention_bounds, within a capture)
+MASK_HOLES = "modelos_b200 attention: a padding mask has padding between real tokens; pad on one side"
 
 
 def read_device_errors(dev: Optional[torch.device] = None, reset: bool = True) -> int:
     """Synchronising read of the error word (bit 1: an index was out of range,
-    bit 2: a bounded wait timed out, bit 4: a row outside the 4-bit cache)."""
+    bit 2: a bounded wait timed out, bit 4: a row outside the 4-bit cache, bit 8:
+    a padding mask with padding between real tokens)."""
     dev = dev or torch.device("cuda", torch.cuda.current_device())
     w = err_word(dev)
     v = int(w.item())
@@ -242,6 +245,8 @@ def check_device_errors(dev: Optional[torch.device] = None):
         raise IndexError("modelos_b200: an embedding index was outside [0, num_rows)")
     if v & DEVERR_CAPACITY:
         raise IndexError("modelos_b200: a token's row was outside the 4-bit cache")
+    if v & DEVERR_MASK:
+        raise ValueError(MASK_HOLES)
     if v & DEVERR_TIMEOUT:
         raise RuntimeError("modelos_b200: a bounded wait inside a kernel timed out")
 

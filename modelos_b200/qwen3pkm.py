@@ -34,6 +34,7 @@ from typing import Iterable, Optional
 import torch
 from torch import nn
 
+from . import _native
 from .attention import MAX_ROWS, KVCache4, window_attention
 from .pkm.memory import HashingMemory
 
@@ -70,12 +71,20 @@ def attention_bounds(attention_mask: torch.Tensor, kv_length: int, kv_offset: Op
     """``[2, B]`` int32: the first real token of each row of a padding mask
     ``[B, tokens]`` among ``kv_length`` columns from ``kv_offset`` on (None: the
     last), and one past the last (equal where a row has none).  Real tokens must
-    be consecutive."""
+    be consecutive: padding between them (a right-padded prompt that goes on) is
+    refused, which waits for the mask; within a capture ``_native.check_device_errors``
+    reports it after a replay."""
     first = attention_mask.shape[1] - kv_length if kv_offset is None else kv_offset
-    m = attention_mask[:, max(first, 0):first + kv_length].to(torch.int32)
+    m = (attention_mask[:, max(first, 0):first + kv_length] != 0).to(torch.int32)
     first = m.argmax(1)
     last = m.shape[1] - m.flip(1).argmax(1)
-    return torch.stack((first, torch.where(m.any(1), last, first))).to(torch.int32)
+    last = torch.where(m.any(1), last, first)
+    holes = (last - first != m.sum(1)).any()
+    if m.is_cuda and torch.cuda.is_current_stream_capturing():
+        _native.err_word(m.device).bitwise_or_(holes.to(torch.int32) * _native.DEVERR_MASK)
+    elif holes:
+        raise ValueError(_native.MASK_HOLES)
+    return torch.stack((first, last)).to(torch.int32)
 
 
 def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None,
@@ -91,6 +100,8 @@ def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     if attention_mask is None:
         return None
     # a column of the mask is a position; it may have columns for tokens to come
+    # (without a cache kv_length is the mask's width, whatever the keys' number)
+    kv_length = min(kv_length, q_offset + q_length - kv_offset)
     if attention_mask.shape[1] < kv_offset + kv_length:
         raise ValueError(f"modelos_b200 attention: the mask has {attention_mask.shape[1]} columns for "
                          f"{kv_offset + kv_length} tokens")

@@ -1,5 +1,6 @@
 """What transformers may hand to this package's attention as mask and
-arguments: right, or refused.  Without a GPU (stand-ins of the kernels)."""
+arguments: right, or refused.  Without a GPU (stand-ins of the kernels), but for
+what a capture does."""
 from __future__ import annotations
 
 import pytest
@@ -16,7 +17,9 @@ WINDOW = dict(use_sliding_window=True, sliding_window=6, max_window_layers=1)  #
 
 
 @pytest.fixture(autouse=True)
-def stand_in(monkeypatch):
+def stand_in(monkeypatch, request):
+    if request.node.get_closest_marker("gpu"):
+        return
     fake_native.install(monkeypatch)
     attnref.install(monkeypatch)
 
@@ -64,3 +67,43 @@ def test_bounds_count_columns_from_the_first_key():
     m = torch.tensor([[0, 0, 1, 1, 1, 1], [1, 1, 1, 1, 1, 0], [0, 0, 0, 0, 0, 1]])
     assert qwen3pkm.attention_bounds(m, 4, 0).tolist() == [[2, 0, 0], [4, 4, 0]]
     assert qwen3pkm.attention_bounds(m, 3, 1).tolist() == [[1, 0, 0], [3, 3, 0]]
+
+
+def test_masks_with_holes_are_refused():
+    """A right-padded prompt that goes on: the padding lies between real tokens."""
+    m = model({})
+    x, mask = ids(2, 6), torch.tensor([[1, 1, 1, 1, 1, 1], [1, 1, 0, 0, 0, 1]])
+    with torch.no_grad():
+        out = m(x[:, :5], attention_mask=mask[:, :5], use_cache=True)
+        with pytest.raises(ValueError, match="between"):
+            m(x[:, 5:], attention_mask=mask, past_key_values=out.past_key_values)
+        with pytest.raises(ValueError, match="between"):
+            m(x, attention_mask=mask, use_cache=False)
+        # behind the last query, and before the first key, they are not seen
+        mask[1] = torch.tensor([1, 1, 1, 0, 0, 1])
+        m(x[:, :5], attention_mask=mask, use_cache=False)
+    holes = torch.tensor([[1, 0, 1, 1]])
+    assert qwen3pkm._attention_mask(1, 1, 2, q_offset=3, kv_offset=2, attention_mask=holes).tolist() == [[0], [2]]
+    with pytest.raises(ValueError, match="between"):
+        qwen3pkm._attention_mask(1, 1, 3, q_offset=2, kv_offset=0, attention_mask=holes)
+    # what is not 0 is real
+    assert qwen3pkm._attention_mask(1, 3, 3, attention_mask=torch.tensor([[0, 2, 255]])).tolist() == [[1], [3]]
+
+
+@pytest.mark.gpu
+def test_a_captured_mask_with_holes_is_reported():
+    """A capture cannot wait for the mask: its replays report it."""
+    from modelos_b200 import _native
+    mask = torch.ones(2, 6, dtype=torch.long, device="cuda")
+    _native.check_device_errors()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        bounds = qwen3pkm._attention_mask(2, 6, 6, attention_mask=mask)
+    graph.replay()
+    _native.check_device_errors()
+    assert bounds.tolist() == [[0, 0], [6, 6]]
+    mask[1, 2] = 0
+    graph.replay()
+    with pytest.raises(ValueError, match="between"):
+        _native.check_device_errors()
+    _native.check_device_errors()
