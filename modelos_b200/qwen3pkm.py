@@ -87,13 +87,32 @@ def attention_bounds(attention_mask: torch.Tensor, kv_length: int, kv_offset: Op
     return torch.stack((first, last)).to(torch.int32)
 
 
+def _alike(f, g) -> bool:
+    """Whether two mask functions are the same code over functions that are
+    alike (numbers that they hold, as a window, may differ)."""
+    def inner(h):
+        for cell in h.__closure__ or ():
+            held = cell.cell_contents
+            yield from (x for x in (held if isinstance(held, (tuple, list)) else (held,)) if callable(x))
+
+    if getattr(f, "__code__", None) is None or f.__code__ is not g.__code__:
+        return False
+    a, b = list(inner(f)), list(inner(g))
+    return len(a) == len(b) and all(map(_alike, a, b))
+
+
 def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, mask_function=None, attention_mask=None,
                     allow_is_causal_skip=True, use_vmap=False, config=None, **kwargs):
     """What transformers hands to ``_attention`` as the mask: None or the
     rows' bounds; causality, window and sinks are the kernels' own."""
-    if use_vmap or not allow_is_causal_skip:
+    from transformers.masking_utils import causal_mask_function, sliding_window_causal_mask_function
+
+    # (chunked, bidirectional and a caller's own masks arrive as a function only)
+    known = mask_function is None or any(
+        _alike(mask_function, f) for f in (causal_mask_function, sliding_window_causal_mask_function(1)))
+    if use_vmap or not allow_is_causal_skip or not known:
         raise ValueError("modelos_b200 attention: only causal and sliding-window masks with padding are implemented "
-                         "(no packed sequences, no overlaid masks, no static cache)")
+                         "(no packed sequences, no chunked, bidirectional or overlaid masks, no static cache)")
     if kv_offset and getattr(config, "attention_sinks", 0):
         raise ValueError("modelos_b200 attention: this cache has dropped the first tokens, which attention_sinks needs; "
                          "pass past_key_values=QuantizedCache(...) or a cache without sliding layers")
@@ -113,6 +132,8 @@ def _attention(module, query, key, value, attention_mask, scaling=None, dropout=
     if dropout:
         raise ValueError("modelos_b200 attention: attention dropout is not implemented")
     sinks = getattr(module.config, "attention_sinks", 0) if sliding_window else 0
+    if attention_mask is not None and (attention_mask.dim() != 2 or attention_mask.dtype != torch.int32):
+        raise ValueError("modelos_b200 attention: masks written out are not implemented; pass a padding mask [batch, tokens]")
     starts, ends = (None, None) if attention_mask is None else attention_mask.unbind()
     if isinstance(key, KVCache4):
         out = key.attend(query, window=sliding_window, sinks=sinks, scale=scaling, starts=starts)

@@ -107,3 +107,32 @@ def test_a_captured_mask_with_holes_is_reported():
     with pytest.raises(ValueError, match="between"):
         _native.check_device_errors()
     _native.check_device_errors()
+
+
+def test_masks_that_are_not_causal_are_refused():
+    """transformers' other masks arrive as a function, not as a tensor."""
+    from transformers import masking_utils as mu
+    m = model(WINDOW)
+    x = torch.zeros(2, 8, 64, dtype=BF)
+    kw = dict(inputs_embeds=x, attention_mask=None, past_key_values=None)
+    assert mu.create_causal_mask(m.config, **kw) is None
+    assert mu.create_sliding_window_causal_mask(m.config, **kw) is None
+    m.config.attention_chunk_size = 4
+    with pytest.raises(ValueError, match="only causal"):
+        mu.create_chunked_causal_mask(m.config, **kw)
+    for f in (mu.bidirectional_mask_function, mu.chunked_causal_mask_function(4, torch.zeros(2, dtype=torch.long)),
+              mu.and_masks(mu.causal_mask_function, lambda b, h, q, k: k != 3),
+              mu.or_masks(mu.causal_mask_function, mu.causal_mask_function),
+              lambda b, h, q, k: k <= q):
+        with pytest.raises(ValueError, match="only causal"):
+            qwen3pkm._attention_mask(2, 8, 8, mask_function=f)
+    for f in (mu.causal_mask_function, mu.sliding_window_causal_mask_function(3)):
+        assert qwen3pkm._attention_mask(2, 8, 8, mask_function=f) is None
+    with pytest.raises(ValueError, match="only causal"):
+        mu.create_bidirectional_mask(m.config, inputs_embeds=x, attention_mask=torch.ones(2, 8))
+
+
+def test_written_out_masks_are_refused():
+    m = model({})
+    with pytest.raises(ValueError, match="padding mask"):
+        m(ids(2, 8), attention_mask=torch.zeros(2, 1, 8, 8, dtype=BF), use_cache=False)
