@@ -127,10 +127,22 @@ def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     return attention_bounds(attention_mask, kv_length, kv_offset)
 
 
-def _attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None, **kwargs):
+# arguments of other models' attention that change its result (score caps, a
+# sink's logit, biases, packed lengths); what else comes along, as position_ids, does not
+_CHANGES = ("softcap", "s_aux", "position_bias", "head_mask", "cu_seq_lens_q", "cu_seq_lens_k")
+
+
+def _attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, sliding_window=None,
+               is_causal=None, **kwargs):
     """transformers' attention interface: ``(output [B, T, heads, D], None)``."""
     if dropout:
         raise ValueError("modelos_b200 attention: attention dropout is not implemented")
+    for name in _CHANGES:
+        if kwargs.get(name) is not None:
+            raise ValueError(f"modelos_b200 attention: {name} is not implemented")
+    # (one query sees all keys either way)
+    if query.shape[2] > 1 and not (getattr(module, "is_causal", True) if is_causal is None else is_causal):
+        raise ValueError("modelos_b200 attention: only causal attention is implemented (is_causal is False)")
     sinks = getattr(module.config, "attention_sinks", 0) if sliding_window else 0
     if attention_mask is not None and (attention_mask.dim() != 2 or attention_mask.dtype != torch.int32):
         raise ValueError("modelos_b200 attention: masks written out are not implemented; pass a padding mask [batch, tokens]")

@@ -136,3 +136,32 @@ def test_written_out_masks_are_refused():
     m = model({})
     with pytest.raises(ValueError, match="padding mask"):
         m(ids(2, 8), attention_mask=torch.zeros(2, 1, 8, 8, dtype=BF), use_cache=False)
+
+
+@pytest.mark.parametrize("what", [dict(softcap=30.0), dict(s_aux=torch.zeros(4)), dict(is_causal=False),
+                                  dict(position_bias=torch.zeros(1)), dict(head_mask=torch.ones(4)),
+                                  dict(cu_seq_lens_q=torch.tensor([0, 4, 8])), dict(cu_seq_lens_k=torch.tensor([0, 4, 8]))])
+def test_arguments_that_change_the_result_are_refused(what):
+    """Score caps, a sink's logit, biases, packed lengths, an encoder's attention."""
+    class Module:
+        config = None
+        is_causal = True
+
+    q, k = torch.zeros(1, 4, 8, 64, dtype=BF), torch.zeros(1, 2, 8, 64, dtype=BF)
+    with pytest.raises(ValueError, match=next(iter(what))):
+        qwen3pkm._attention(Module, q, k, k, None, **what)
+    none = {name: None for name in what}
+    out, _ = qwen3pkm._attention(Module, q, k, k, None, position_ids=torch.zeros(1, 8), use_cache=True, **none)
+    assert out.shape == (1, 8, 4, 64)
+
+
+def test_modules_that_are_not_causal_are_refused():
+    class Module:
+        config = None
+        is_causal = False
+
+    q = torch.zeros(1, 4, 8, 64, dtype=BF)
+    with pytest.raises(ValueError, match="is_causal"):
+        qwen3pkm._attention(Module, q, q, q, None)
+    qwen3pkm._attention(Module, q, q, q, None, is_causal=True)
+    qwen3pkm._attention(Module, q[:, :, :1], q, q, None)  # one query sees all keys either way
