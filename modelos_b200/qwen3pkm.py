@@ -124,7 +124,10 @@ def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
     if attention_mask.shape[1] < kv_offset + kv_length:
         raise ValueError(f"modelos_b200 attention: the mask has {attention_mask.shape[1]} columns for "
                          f"{kv_offset + kv_length} tokens")
-    return attention_bounds(attention_mask, kv_length, kv_offset)
+    bounds = attention_bounds(attention_mask, kv_length, kv_offset)
+    # where all queries are padding, nothing is visible: KVCache4.attend takes no ends
+    bounds[0].masked_fill_(bounds[1] <= kv_length - q_length, kv_length)
+    return bounds
 
 
 # arguments of other models' attention that change its result (score caps, a

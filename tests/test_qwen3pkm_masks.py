@@ -165,3 +165,23 @@ def test_modules_that_are_not_causal_are_refused():
         qwen3pkm._attention(Module, q, q, q, None)
     qwen3pkm._attention(Module, q, q, q, None, is_causal=True)
     qwen3pkm._attention(Module, q[:, :, :1], q, q, None)  # one query sees all keys either way
+
+
+@pytest.mark.parametrize("kw", [{}, WINDOW])
+def test_rows_whose_tokens_are_all_padding_over_the_4_bit_cache(kw):
+    """A row without real tokens, and one that has ended: as over the 16-bit cache,
+    their tokens see nothing."""
+    m = model(kw)
+    x, mask = ids(3, 12), torch.ones(3, 12, dtype=torch.long)
+    mask[1] = 0
+    mask[2, 8:] = 0
+    logits = []
+    with torch.no_grad():
+        for cache in (None, qwen3pkm.QuantizedCache(m.config, 16)):
+            out = m(x[:, :8], attention_mask=mask[:, :8], past_key_values=cache, use_cache=True)
+            steps = []
+            for a, b in ((8, 9), (9, 12)):
+                out = m(x[:, a:b], attention_mask=mask[:, :b], past_key_values=out.past_key_values)
+                steps.append(out.logits[1:])
+            logits.append(torch.cat(steps, 1))
+    assert torch.equal(*logits)  # (the attention's output is 0 in every layer)
