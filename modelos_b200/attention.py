@@ -45,10 +45,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     ``D ** -0.5``.
 
     Returns [B, heads, Tq, D], laid out in memory as ``q`` is ([B, T, heads,
-    D] or contiguous).  Differentiable once in q, k and v; results are
-    deterministic.  May be captured into a graph, also with its backward pass:
-    refused (``RuntimeError``) while an eager graph of the default stream holds
-    leaves among q, k and v, whose gradients would be accumulated there.
+    D] or contiguous).  Differentiable once in q, k and v, backwards (tensors
+    with a forward-mode tangent are refused); results are deterministic.  May be
+    captured into a graph, also with its backward pass: refused
+    (``RuntimeError``) while an eager graph of the default stream holds leaves
+    among q, k and v, whose gradients would be accumulated there.
     """
     return _native.attention().window_attention(q, k, v, window or 0, sinks, scale, starts, ends)
 

@@ -28,6 +28,12 @@ void need_cuda(const Tensor& t) {
   TORCH_CHECK(t.is_cuda(), "modelos_b200 kernels need CUDA tensors (there is no CPU path)");
 }
 
+// A tensor with a forward-mode tangent, which the kernels would drop.
+void no_dual(const Tensor& t) {
+  TORCH_CHECK(!t.unsafeGetTensorImpl()->_fw_grad(0, t).defined(),
+              "modelos_b200 attention: forward-mode derivatives are not implemented");
+}
+
 void check(int rc, const char* name) {
   TORCH_CHECK(rc == PKM_OK, name, " failed (", pkm_status_string(rc), "): ", pkm_last_error());
 }
@@ -162,6 +168,7 @@ Tensor window_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, in
   REFUSE(k0.size(0) == B && k0.size(3) == D, "q and k disagree in batch or head_dim");
   REFUSE(q0.scalar_type() == k0.scalar_type() && q0.scalar_type() == v0.scalar_type(), "q, k and v must share a type");
   REFUSE(half_type(q0), "only bf16 and fp16 are implemented");
+  for (const Tensor* t : {&q0, &k0, &v0}) no_dual(*t);
   need_cuda(q0);
   need_cuda(k0);
   need_cuda(v0);
@@ -199,6 +206,8 @@ void kv4_write(const Tensor& k0, const Tensor& v0, const OptTensor& at, int64_t 
   REFUSE(k0.size(0) == B && k0.size(1) == Hk && k0.size(3) == D, "k does not fit the cache");
   REFUSE(k0.scalar_type() == kp.scalar_type() && v0.scalar_type() == kp.scalar_type(),
          "k and v must have the cache's type");
+  no_dual(k0);
+  no_dual(v0);
   need_cuda(k0);
   need_cuda(v0);
   REFUSE(k0.device() == kc.device() && v0.device() == kc.device(), "k and v must be on the cache's device");
@@ -234,6 +243,7 @@ Tensor kv4_attend(const Tensor& q0, const Tensor& kc, const Tensor& kp, const Te
   const int64_t B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = 2 * kc.size(3);
   REFUSE(q0.dim() == 4 && q0.size(0) == B && q0.size(3) == D, "q does not fit the cache");
   REFUSE(q0.scalar_type() == kp.scalar_type(), "q must have the cache's type");
+  no_dual(q0);
   need_cuda(q0);
   REFUSE(q0.device() == kc.device(), "q must be on the cache's device");
   REFUSE(Hk > 0 && q0.size(1) % Hk == 0, "heads must be a multiple of kv_heads");
