@@ -194,6 +194,17 @@ Tensor window_attention(const Tensor& q0, const Tensor& k0, const Tensor& v0, in
 // ---------------------------------------------------------------------------
 // the 4-bit cache: codes [B, Hk, cap, D/2], params [B, Hk, cap, D/32, 2]
 // ---------------------------------------------------------------------------
+// The cache's tensors are attributes that a caller can replace.
+void check_cache(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp) {
+  bool ok = kc.dim() == 4 && kc.scalar_type() == at::kByte && (kc.size(3) == 32 || kc.size(3) == 64) &&
+            vc.scalar_type() == at::kByte && vc.sizes() == kc.sizes() && kp.dim() == 5 && half_type(kp) &&
+            vp.scalar_type() == kp.scalar_type() && vp.sizes() == kp.sizes();
+  for (int i = 0; i < 3; ++i) ok = ok && kp.size(i) == kc.size(i);
+  ok = ok && kp.size(3) == kc.size(3) / 16 && kp.size(4) == 2;
+  for (const Tensor* t : {&kc, &kp, &vc, &vp}) ok = ok && t->is_contiguous() && t->device() == kc.device();
+  REFUSE(ok, "the cache's codes and params do not fit together");
+}
+
 // Row numbers: a tensor [batch], or one number for all (-1: there is a tensor).
 void check_rows(int64_t at0, const OptTensor& at, int64_t n, int64_t cap) {
   REFUSE(at || (at0 >= 0 && at0 <= cap - n), "rows outside the cache");
@@ -201,6 +212,7 @@ void check_rows(int64_t at0, const OptTensor& at, int64_t n, int64_t cap) {
 
 void kv4_write(const Tensor& k0, const Tensor& v0, const OptTensor& at, int64_t at0, const Tensor& kc, const Tensor& kp,
                const Tensor& vc, const Tensor& vp) {
+  check_cache(kc, kp, vc, vp);
   const int64_t B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = 2 * kc.size(3);
   REFUSE(k0.dim() == 4 && k0.sizes() == v0.sizes(), "k and v must be [batch, kv_heads, tokens, head_dim] of one shape");
   REFUSE(k0.size(0) == B && k0.size(1) == Hk && k0.size(3) == D, "k does not fit the cache");
@@ -224,6 +236,7 @@ void kv4_write(const Tensor& k0, const Tensor& v0, const OptTensor& at, int64_t 
 
 std::tuple<Tensor, Tensor> kv4_read(const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp,
                                     const OptTensor& at, int64_t at0, int64_t n) {
+  check_cache(kc, kp, vc, vp);
   const int64_t B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = 2 * kc.size(3);
   REFUSE(n >= 0, "count must not be negative");
   need_cuda(kc);
@@ -240,7 +253,11 @@ std::tuple<Tensor, Tensor> kv4_read(const Tensor& kc, const Tensor& kp, const Te
 Tensor kv4_attend(const Tensor& q0, const Tensor& kc, const Tensor& kp, const Tensor& vc, const Tensor& vp,
                   int64_t window, int64_t sinks, std::optional<double> scale, const OptTensor& starts,
                   const Tensor& lengths) {
+  check_cache(kc, kp, vc, vp);
   const int64_t B = kc.size(0), Hk = kc.size(1), cap = kc.size(2), D = 2 * kc.size(3);
+  REFUSE(lengths.dim() == 1 && lengths.size(0) == B && lengths.scalar_type() == at::kInt && lengths.is_contiguous() &&
+             lengths.device() == kc.device(),
+         "lengths must be int32 [batch] on the cache's device");
   REFUSE(q0.dim() == 4 && q0.size(0) == B && q0.size(3) == D, "q does not fit the cache");
   REFUSE(q0.scalar_type() == kp.scalar_type(), "q must have the cache's type");
   no_dual(q0);
