@@ -57,7 +57,7 @@ static AttnArgs attn_args(int64_t B, int64_t Hq, int64_t Hk, int64_t Tq, int64_t
 
 using namespace pkm;
 
-// Partial outputs (with what their rounding left) and sums of a split.
+// Partial outputs and sums of a split, in 32 bits.
 static size_t attn_fwd_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t D, int splits) {
   return splits > 1 ? (size_t)splits * B * Hq * Tq * (4 * D + sizeof(float)) : 0;
 }

@@ -453,13 +453,14 @@ struct DkvItem {
 // Rows of TMEM are keys.  TMEM: S^T (columns 0; P^T over it, the halves of
 // the block's queries at 0 and 64), dP^T (128; dS^T over it), dv (256), dk
 // (256 + DP).
-template <typename T, int DP>
+// FAR: some items are parts, stored in 32 bits (compiled apart: with both ways to
+// store in one kernel the compiler spills registers).
+template <typename T, int DP, bool FAR>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo,
                     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const __grid_constant__ CUtensorMap tdk, const __grid_constant__ CUtensorMap tdv,
                     const __grid_constant__ CUtensorMap tpk, const __grid_constant__ CUtensorMap tpv,
-                    const __grid_constant__ CUtensorMap tpk_lo, const __grid_constant__ CUtensorMap tpv_lo,
                     const AttnBwdArgs g) {
   const AttnArgs& a = g.f;
   using F = BwTile<DP>;
@@ -791,12 +792,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       // the first half of the threads stores dv, the second dk
       const uint32_t acc = (half ? t_dk : t_dv) + lanes;
       const float f = half ? a.scale : 1.f;
-      const bool parts = w.slot >= 0;
-      const CUtensorMap* to = half ? (parts ? &tpk : &tdk) : (parts ? &tpv : &tdv);
-      if (!w.none)
-        store_tile<T, DP>(acc, so + half * AT_BOX, rl, f, real, w.count > 0, to, parts ? 0 : w.j0, parts ? 0 : w.hk,
-                          parts ? w.slot : w.b, 1 + half, leader, acc_empty, 0,
-                          parts ? (half ? &tpk_lo : &tpv_lo) : nullptr);
+      if (FAR && w.slot >= 0)
+        store_part<DP>(acc, so + half * AT_BOX, rl, f, real, w.count > 0, half ? &tpk : &tpv, a.D, 0, 0, w.slot,
+                       1 + half, leader, acc_empty);
+      else if (!w.none)
+        store_tile<T, DP>(acc, so + half * AT_BOX, rl, f, real, w.count > 0, half ? &tdk : &tdv, w.j0, w.hk, w.b,
+                          1 + half, leader, acc_empty);
     }
     if (leader) bulk_wait_all();
   }
@@ -807,10 +808,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 }
 
 // The parts of the key tiles that hold sinks, summed in their order: 16 lanes a
-// row, dk and dv in turn.
+// row, dk and dv in turn.  Parts are in 32 bits: a part may leave fp16's range
+// where the sum does not.
 struct FarArgs {
-  const void* hi[2];  // dk, dv: [slots, 128, D], and what their rounding left
-  const void* lo[2];
+  const float* part[2];  // dk, dv: [slots, 128, D]
 };
 template <typename T>
 __global__ void __launch_bounds__(256) attn_far_join_kernel(const AttnBwdArgs g, const FarArgs f) {
@@ -825,12 +826,13 @@ __global__ void __launch_bounds__(256) attn_far_join_kernel(const AttnBwdArgs g,
   const int side = blockIdx.y;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int p = 0; p <= g.far_parts; ++p) {
-    const int64_t at = (((int64_t)tile * (g.far_parts + 1) + p) * AT_T + rl) * a.D + d;
-    float hi[8], lo[8];
-    VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(f.hi[side]) + at), hi);
-    VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(f.lo[side]) + at), lo);
+    float u[8];
+    const float4* at = reinterpret_cast<const float4*>(
+        f.part[side] + (((int64_t)tile * (g.far_parts + 1) + p) * AT_T + rl) * a.D + d);
+    *reinterpret_cast<float4*>(u) = at[0];
+    *reinterpret_cast<float4*>(u + 4) = at[1];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) sum[y] += hi[y] + lo[y];
+    for (int y = 0; y < 8; ++y) sum[y] += u[y];
   }
   const Strides3& s = side ? g.sdv : g.sdk;
   *reinterpret_cast<uint4*>(static_cast<T*>(side ? g.dv : g.dk) + b * s.b + hk * s.h + (int64_t)row * s.t + d) =
@@ -850,7 +852,7 @@ size_t attn_bwd_far(AttnBwdArgs& g) {
   if (all < 2 * near || 2 * all * num_sms() < heads * (tiles * near + all)) return 0;
   g.far_tiles = (a.sinks - 1) / AT_T + 2;
   g.far_parts = (int)std::min<int64_t>(16, (all - 1) / near);
-  return (size_t)heads * g.far_tiles * (g.far_parts + 1) * AT_T * a.D * 2 * 4;
+  return (size_t)heads * g.far_tiles * (g.far_parts + 1) * AT_T * a.D * 2 * sizeof(float);
 }
 
 template <typename T, int DP>
@@ -859,10 +861,11 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
   constexpr int dt = DtOf<T>::value;
   constexpr int smem = BwTile<DP>::SMEM;
   // (before the tensor maps: it makes the device's context current on this thread)
+  const auto dkv = g.far_tiles ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>;
   if (cudaFuncSetAttribute(attn_dq_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
-      cudaFuncSetAttribute(attn_dkv_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_cuda("cudaFuncSetAttribute(attn_bwd)");
-  CUtensorMap tq{}, tdo{}, tk, tv, tdq{}, tdk, tdv, tp[4]{};
+  CUtensorMap tq{}, tdo{}, tk, tv, tdq{}, tdk, tdv, tp[2]{};
   int rc;
   if ((rc = attn_tmap(&tk, a.k, dt, a.sk, a.B, a.Hk, a.Tk, a.D)) ||
       (rc = attn_tmap(&tv, a.v, dt, a.sv, a.B, a.Hk, a.Tk, a.D)) ||
@@ -873,12 +876,13 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
                    (rc = attn_tmap(&tdo, g.dout, dt, g.sdo, a.B, a.Hq, a.Tq, a.D)) ||
                    (rc = attn_tmap(&tdq, g.dq, dt, g.sdq, a.B, a.Hq, a.Tq, a.D))))
     return rc;
-  // partial sums: dk, dv, what the rounding of each left
+  // partial sums: dk, dv
   const int64_t slots = (int64_t)a.B * a.Hk * g.far_tiles * (g.far_parts + 1);
-  T* part[4];
-  for (int i = 0; i < 4 && slots; ++i) {
-    part[i] = static_cast<T*>(partials) + i * slots * AT_T * a.D;
-    if ((rc = attn_tmap(&tp[i], part[i], dt, Strides3{(int64_t)AT_T * a.D, 0, a.D}, slots, 1, AT_T, a.D))) return rc;
+  FarArgs far{};
+  for (int i = 0; i < 2 && slots; ++i) {
+    far.part[i] = static_cast<const float*>(partials) + i * slots * AT_T * a.D;
+    if ((rc = attn_tmap(&tp[i], far.part[i], PKM_DT_F32, Strides3{(int64_t)AT_T * a.D, 0, a.D}, slots, 1, AT_T, a.D)))
+      return rc;
   }
   const int64_t gq = (int64_t)((a.Tq + AT_T - 1) / AT_T) * a.G * a.B * a.Hk;
   const int64_t gk = ((int64_t)((a.Tk + AT_T - 1) / AT_T) + g.far_tiles * g.far_parts) * a.B * a.Hk;
@@ -892,11 +896,9 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
     attn_dq_kernel<T, DP><<<(unsigned)std::min<int64_t>(gq, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdq, g);
   }
   if ((rc = check_cuda("attn_dq"))) return rc;
-  attn_dkv_kernel<T, DP><<<(unsigned)std::min<int64_t>(gk, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdk, tdv,
-                                                                                             tp[0], tp[1], tp[2], tp[3], g);
+  dkv<<<(unsigned)std::min<int64_t>(gk, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdk, tdv, tp[0], tp[1], g);
   if ((rc = check_cuda("attn_dkv")) || !slots) return rc;
-  const FarArgs f{{part[0], part[1]}, {part[2], part[3]}};
-  attn_far_join_kernel<T><<<dim3((unsigned)((int64_t)a.B * a.Hk * g.far_tiles * (AT_T / 16)), 2), 256, 0, st>>>(g, f);
+  attn_far_join_kernel<T><<<dim3((unsigned)((int64_t)a.B * a.Hk * g.far_tiles * (AT_T / 16)), 2), 256, 0, st>>>(g, far);
   return check_cuda("attn_far_join");
 }
 

@@ -98,7 +98,9 @@ struct FwItem {
   }
 };
 
-template <typename T, int DP>
+// PART: items are parts of a split, stored in 32 bits (compiled apart: with both
+// ways to store in one kernel the compiler spills registers).
+template <typename T, int DP, bool PART>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tout,
@@ -424,12 +426,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       // which rows see something goes by position (a row sees itself at least),
       // not by their sum, which a NaN or an infinite score makes NaN; a part of a
       // split may have nothing for such a row
-      const bool some = row < a.Tq && pr >= 0 && pr < w.len && (a.splits == 1 || l != 0.f);
+      const bool some = row < a.Tq && pr >= 0 && pr < w.len && (!PART || l != 0.f);
       if (a.lse && row < a.Tq)
         a.lse[((int64_t)w.ob * a.Hq + h) * a.Tq + row] = some ? (m + log2f(l)) * AT_LN2 : -INFINITY;
       const float inv = some ? 1.f / l : 0.f;
-      store_tile<T, DP>(to, so + i * AT_BOX, rl, inv, some, w.count > 0, &tout, r0, h, w.ob, 1 + i, leader, &o_empty[i],
-                        0, a.out_lo ? &tlo : nullptr);
+      if constexpr (PART)
+        store_part<DP>(to, so + i * AT_BOX, rl, inv, some, w.count > 0, &tout, a.D, r0, h, w.ob, 1 + i, leader,
+                       &o_empty[i]);
+      else
+        store_tile<T, DP>(to, so + i * AT_BOX, rl, inv, some, w.count > 0, &tout, r0, h, w.ob, 1 + i, leader,
+                          &o_empty[i], 0, a.out_lo ? &tlo : nullptr);
     }
     if (leader) bulk_wait_all();
   }
@@ -442,17 +448,18 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 int attn_tmap(CUtensorMap* m, const void* p, int dtype, const Strides3& s, int64_t B, int64_t H, int64_t T, int64_t D,
               int rows) {
   // the stride of a dimension of size 1 is never used, but must be a valid one
-  auto bytes = [&](int64_t st) { return (uint64_t)std::max<int64_t>(st * 2, 16); };
+  const int size = dtype_size(dtype);
+  auto bytes = [&](int64_t st) { return (uint64_t)std::max<int64_t>(st * size, 16); };
   return make_tmap_4d(m, p, dtype, (uint64_t)D, (uint64_t)T, (uint64_t)H, (uint64_t)B, bytes(s.t), bytes(s.h),
-                      bytes(s.b), 64, (uint32_t)rows);
+                      bytes(s.b), 128u / size, (uint32_t)rows);
 }
 
 // The parts of a split joined in their order: 16 lanes a row, as 128-bit pieces.
+// Parts are in 32 bits: a part's rounding would come on top of the output's.
 // A part whose sum is NaN makes the row NaN (the maximum alone would pass over it).
 struct JoinArgs {
-  const void* hi;  // [splits, B, Hq, Tq, D], and lo, lse
-  const void* lo;
-  const float* lse;
+  const float* part;  // [splits, B, Hq, Tq, D]
+  const float* lse;   // [splits, B, Hq, Tq]
   AttnArgs a;
 };
 template <typename T>
@@ -479,12 +486,12 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const JoinArgs j, FastDi
       const float w = expf(j.lse[s * rows + r] - m);  // (NaN where every score is -inf: 0 / 0)
       sum += w;
       if (d < a.D) {
-        float hi[8], lo[8];
-        const int64_t at = (s * rows + r) * a.D + d;
-        VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(j.hi) + at), hi);
-        VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(j.lo) + at), lo);
+        float u[8];
+        const float4* at = reinterpret_cast<const float4*>(j.part + (s * rows + r) * a.D + d);
+        *reinterpret_cast<float4*>(u) = at[0];
+        *reinterpret_cast<float4*>(u + 4) = at[1];
 #pragma unroll
-        for (int y = 0; y < 8; ++y) o[y] = fmaf(w, hi[y] + lo[y], o[y]);
+        for (int y = 0; y < 8; ++y) o[y] = fmaf(w, u[y], o[y]);
       }
     }
     const float inv = 1.f / sum;
@@ -522,52 +529,56 @@ int attn_fwd_splits(int64_t B, int64_t Hk, int64_t G, int64_t Tq, int64_t Tk, in
   return (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / std::max<int64_t>(items, 1), keys / (4 * AT_T), 16}));
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool PART>
 static int attn_fwd_go(const AttnArgs& a0, void* workspace, cudaStream_t st) {
   AttnArgs a = a0;
   JoinArgs join{};
   Strides3 so = a.so;
   const int64_t rows = (int64_t)a.B * a.Hq * a.Tq;
-  if (a.splits > 1) {
+  if (PART) {
     // the parts' outputs take the output's place
     join.a = a0;
-    join.hi = a.out = workspace;
-    a.out_lo = static_cast<T*>(workspace) + a.splits * rows * a.D;
-    join.lo = a.out_lo;
-    a.lse = reinterpret_cast<float*>(static_cast<T*>(a.out_lo) + a.splits * rows * a.D);
-    join.lse = a.lse;
+    a.out = workspace;
+    a.out_lo = nullptr;
+    join.part = static_cast<const float*>(workspace);
+    join.lse = a.lse = static_cast<float*>(workspace) + a.splits * rows * a.D;
     so = Strides3{(int64_t)a.Hq * a.Tq * a.D, (int64_t)a.Tq * a.D, a.D};
   }
   constexpr int dt = DtOf<T>::value;
   // (also makes the device's context current: a tensor map cannot be encoded
   // on a thread that has made no CUDA call yet, such as autograd's)
-  if (cudaFuncSetAttribute(attn_fwd_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, FwTile<DP>::SMEM) !=
-      cudaSuccess)
+  if (cudaFuncSetAttribute(attn_fwd_kernel<T, DP, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           FwTile<DP>::SMEM) != cudaSuccess)
     return check_cuda("cudaFuncSetAttribute(attn_fwd)");
   CUtensorMap tq, tk, tv, tout, tlo{};
   int rc;
   if ((rc = attn_tmap(&tq, a.q, dt, a.sq, a.B, a.Hq, a.Tq, a.D)) ||
       (rc = attn_tmap(&tk, a.k, dt, a.sk, a.B, a.Hk, a.Tk, a.D)) ||
       (rc = attn_tmap(&tv, a.v, dt, a.sv, a.B, a.Hk, a.Tk, a.D)) ||
-      (rc = attn_tmap(&tout, a.out, dt, so, (int64_t)a.B * a.splits, a.Hq, a.Tq, a.D)) ||
-      (a.out_lo && (rc = attn_tmap(&tlo, a.out_lo, dt, so, (int64_t)a.B * a.splits, a.Hq, a.Tq, a.D))))
+      (rc = attn_tmap(&tout, a.out, PART ? PKM_DT_F32 : dt, so, (int64_t)a.B * a.splits, a.Hq, a.Tq, a.D)) ||
+      (a.out_lo && (rc = attn_tmap(&tlo, a.out_lo, dt, so, a.B, a.Hq, a.Tq, a.D))))
     return rc;
   const int64_t tiles = (int64_t)((a.Tq + AT_T - 1) / AT_T) * a.G;
   const int64_t items = (tiles + 1) / 2 * a.B * a.Hk * a.splits;
   if (items > INT32_MAX / 2) return fail(PKM_ERR_UNSUPPORTED, "too many rows");
   const int grid = (int)std::min<int64_t>(items, num_sms());
-  attn_fwd_kernel<T, DP><<<grid, FW_THREADS, FwTile<DP>::SMEM, st>>>(tq, tk, tv, tout, tlo, a);
-  if ((rc = check_cuda("attn_fwd")) || a.splits == 1) return rc;
+  attn_fwd_kernel<T, DP, PART><<<grid, FW_THREADS, FwTile<DP>::SMEM, st>>>(tq, tk, tv, tout, tlo, a);
+  if ((rc = check_cuda("attn_fwd")) || !PART) return rc;
   attn_join_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(join, FastDiv((uint32_t)a.Tq),
                                                                    FastDiv((uint32_t)a.Hq));
   return check_cuda("attn_join");
 }
 
+template <typename T, int DP>
+static int attn_fwd_parts(const AttnArgs& a, void* workspace, cudaStream_t st) {
+  return a.splits > 1 ? attn_fwd_go<T, DP, true>(a, workspace, st) : attn_fwd_go<T, DP, false>(a, workspace, st);
+}
+
 int attn_fwd_launch(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st) {
   if (dtype == PKM_DT_BF16)
-    return a.D > 64 ? attn_fwd_go<__nv_bfloat16, 128>(a, workspace, st)
-                    : attn_fwd_go<__nv_bfloat16, 64>(a, workspace, st);
-  return a.D > 64 ? attn_fwd_go<__half, 128>(a, workspace, st) : attn_fwd_go<__half, 64>(a, workspace, st);
+    return a.D > 64 ? attn_fwd_parts<__nv_bfloat16, 128>(a, workspace, st)
+                    : attn_fwd_parts<__nv_bfloat16, 64>(a, workspace, st);
+  return a.D > 64 ? attn_fwd_parts<__half, 128>(a, workspace, st) : attn_fwd_parts<__half, 64>(a, workspace, st);
 }
 
 }  // namespace pkm

@@ -143,7 +143,7 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Tensor map over [B, H, T, D] with boxes of 64 channels x `rows` tokens.
+// Tensor map over [B, H, T, D] with boxes of 128 bytes of channels x `rows` tokens.
 int attn_tmap(CUtensorMap* m, const void* p, int dtype, const Strides3& s, int64_t B, int64_t H, int64_t T, int64_t D,
               int rows = AT_T);
 
@@ -275,6 +275,45 @@ __device__ __forceinline__ void store_tile(uint32_t taddr, unsigned char* box, i
         tma_store_4d(part ? lo : map, box, x0 + x, y, z, w);
         bulk_commit_group();
       }
+    }
+  }
+}
+
+// The same for a partial result, in 32 bits: 32 channels at a time, up to the
+// last of the tensor's D (a box starts inside the tensor).
+template <int DP>
+__device__ __forceinline__ void store_part(uint32_t taddr, unsigned char* box, int row, float f, bool some, bool have,
+                                           const CUtensorMap* map, int D, int y, int z, int w, int id, bool leader,
+                                           uint64_t* drained) {
+  const uint32_t sb = smem_u32(box) + row * 128;
+  const int channels = min(D, DP);
+#pragma unroll 1
+  for (int x = 0; x < channels; x += 32) {
+    if (leader) bulk_wait_read_all();
+    named_sync(id, AT_T);
+    uint32_t o[32];
+    if (have) {
+      tmem_ld_32x32b_x32(taddr + x, o);
+      tmem_ld_wait();
+      if (x + 32 >= channels) {
+        tc_fence_before();
+        mbar_arrive(drained);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t v[4] = {0, 0, 0, 0};
+      if (have && some) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __float_as_uint(__uint_as_float(o[c * 4 + e]) * f);
+      }
+      sts128(sb + ((c ^ (row & 7)) << 4), v[0], v[1], v[2], v[3]);
+    }
+    fence_proxy_async_smem();
+    named_sync(id, AT_T);
+    if (leader) {
+      tma_store_4d(map, box, x, y, z, w);
+      bulk_commit_group();
     }
   }
 }

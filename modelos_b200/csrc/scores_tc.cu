@@ -291,13 +291,16 @@ int make_tmap_4d(CUtensorMap* map, const void* base, int dtype, uint64_t cols, u
                  uint64_t s1, uint64_t s2, uint64_t s3, uint32_t box_cols, uint32_t box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(PKM_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-  if (dtype != PKM_DT_BF16 && dtype != PKM_DT_F16) return fail(PKM_ERR_INVALID_ARG, "tensor map dtype");
+  if (!valid_dtype(dtype)) return fail(PKM_ERR_INVALID_ARG, "tensor map dtype");
   const cuuint64_t dims[4] = {cols, d1, d2, d3};
   const cuuint64_t strides[3] = {s1, s2, s3};
   const cuuint32_t box[4] = {box_cols, box_rows, 1, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = dtype == PKM_DT_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == PKM_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const CUresult r =
-      fn(map, dtype == PKM_DT_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+      fn(map, type, 4,
          const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PKM_ERR_INVALID_ARG, "cuTensorMapEncodeTiled rejected the operand");

@@ -270,7 +270,7 @@ int make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t cols, uint64_
 int make_tmap_2d(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t rows,
                  uint64_t row_stride_bytes, uint32_t box_cols, uint32_t box_rows, int swizzle_bytes);
 
-// 4-D map over 16-bit elements [d3, d2, d1, cols], strides in bytes of d1,
+// 4-D map over 16-bit or fp32 elements [d3, d2, d1, cols], strides in bytes of d1,
 // d2, d3; boxes of box_cols x box_rows (d1) x 1 x 1, 128-byte swizzle.
 int make_tmap_4d(CUtensorMap* map, const void* base, int dtype, uint64_t cols, uint64_t d1, uint64_t d2, uint64_t d3,
                  uint64_t s1, uint64_t s2, uint64_t s3, uint32_t box_cols, uint32_t box_rows);
