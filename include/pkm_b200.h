@@ -582,9 +582,11 @@ PKM_API int pkm_batchnorm_bwd(const void* dy, const void* x, int x_dtype, int64_
  * backward pass pkm_attn_bwd_workspace(); 16-byte aligned, free for reuse once
  * the call's work on the stream is done.
  * The backward pass reads out, out_lo and lse as the forward pass wrote them, sums
- * dk and dv over the query heads of a key/value head in a fixed order, and
- * uses no atomics: results are deterministic.  dq, dk and dv may not overlap
- * the inputs.
+ * dk and dv over the query heads of a key/value head in a fixed order:
+ * results are deterministic.  In fp16, P and P (dP - delta) are held times
+ * powers of two between their products, so that dout's size does not matter
+ * while the gradients themselves stay within the type.  dq, dk and dv may not
+ * overlap the inputs.
  */
 PKM_API int pkm_attn_fwd_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D,
                                    int64_t window, int64_t sinks, size_t* bytes);

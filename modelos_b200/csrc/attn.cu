@@ -109,9 +109,13 @@ extern "C" int pkm_attn_fwd(const void* q, const int64_t* q_strides, const void*
   return attn_fwd_launch(a, dtype, workspace, st);
 }
 
-// delta, then the partial sums of key tiles that hold sinks.
-static size_t attn_bwd_delta(int64_t B, int64_t Hq, int64_t Tq) {
+// delta and the rows' norms, the heads' largest norms, then the partial sums of
+// key tiles that hold sinks.
+static size_t attn_bwd_rows(int64_t B, int64_t Hq, int64_t Tq) {
   return ((size_t)B * Hq * Tq * sizeof(float) + 255) / 256 * 256;
+}
+static size_t attn_bwd_stats(int64_t B, int64_t Hq, int64_t Hk, int64_t Tq) {
+  return 2 * attn_bwd_rows(B, Hq, Tq) + (size_t)B * Hk * 2 * AT_PEAK * sizeof(float);
 }
 
 extern "C" int pkm_attn_bwd_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t Tq, int64_t Tk, int64_t D,
@@ -119,7 +123,7 @@ extern "C" int pkm_attn_bwd_workspace(int64_t B, int64_t Hq, int64_t Hk, int64_t
   if (!bytes) return fail(PKM_ERR_INVALID_ARG, "null bytes");
   const int rc = attn_check(PKM_DT_BF16, B, Hq, Hk, Tq, Tk, D, 1.0, window, sinks);
   if (rc) return rc;
-  *bytes = attn_bwd_delta(B, Hq, Tq);
+  *bytes = attn_bwd_stats(B, Hq, Hk, Tq);
   if (B && Hq && Tk) {
     AttnBwdArgs g{};
     g.f = attn_args(B, Hq, Hk, Tq, Tk, D, 1.0, window, sinks, nullptr, nullptr, nullptr);
@@ -152,7 +156,7 @@ extern "C" int pkm_attn_bwd(const void* q, const int64_t* q_strides, const void*
              (rc = attn_layout(dq, dq_strides, B, Hq, Tq, "dq", &g.sdq))))
     return rc;
   if (Tq && (!lse || !out_lo || !aligned16(out_lo))) return fail(PKM_ERR_INVALID_ARG, "null lse or out_lo");
-  const size_t need = attn_bwd_delta(B, Hq, Tq) + attn_bwd_far(g);
+  const size_t stats = attn_bwd_stats(B, Hq, Hk, Tq), need = stats + attn_bwd_far(g);
   if (need && !aligned16(workspace)) return fail(PKM_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
   if (workspace_bytes < need || (need && !workspace))
     return fail(PKM_ERR_WORKSPACE, "pkm_attn_bwd: workspace smaller than pkm_attn_bwd_workspace()");
@@ -166,7 +170,10 @@ extern "C" int pkm_attn_bwd(const void* q, const int64_t* q_strides, const void*
   g.dq = dq;
   g.dk = dk;
   g.dv = dv;
-  g.delta = static_cast<float*>(workspace);
+  char* ws = static_cast<char*>(workspace);
+  g.delta = reinterpret_cast<float*>(ws);
+  g.norms = reinterpret_cast<float*>(ws + attn_bwd_rows(B, Hq, Tq));
+  g.peaks = reinterpret_cast<float*>(ws + 2 * attn_bwd_rows(B, Hq, Tq));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return attn_bwd_launch(g, dtype, static_cast<char*>(workspace) + attn_bwd_delta(B, Hq, Tq), st);
+  return attn_bwd_launch(g, dtype, ws + stats, st);
 }

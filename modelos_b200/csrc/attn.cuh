@@ -39,6 +39,8 @@ struct AttnArgs {
   uint32_t* err;
 };
 
+constexpr int AT_PEAK = 32;  // a cache line: the updates of different heads do not queue
+
 struct AttnBwdArgs {
   AttnArgs f;
   const void* dout;
@@ -47,6 +49,10 @@ struct AttnBwdArgs {
   void* dv;
   Strides3 sdo, sdq, sdk, sdv;
   float* delta;  // [B, Hq, Tq]: sum over the channels of dout * out
+  // fp16 only: the norms of dout's rows [B, Hq, Tq], and for each key/value head
+  // the largest of them and of v's rows [2][B, Hk], AT_PEAK numbers apart
+  float* norms;
+  float* peaks;
   // key tiles that hold sinks are seen by all later queries: those behind the
   // window are items of their own, `far_parts` for each of up to `far_tiles`
   // such tiles of a head (0: no such items), joined afterwards

@@ -4,7 +4,7 @@
 //   delta = sum_d dout out,
 //   dq = scale dS k,  dk = scale dS^T q,  dv = P^T dout
 //
-// Two persistent kernels without atomics, so that sums have a fixed order:
+// Two persistent kernels that add nothing by atomics, so that sums have a fixed order:
 // attn_dq walks the key blocks that a tile of 128 query rows sees (3 products
 // a block), attn_dkv walks the query blocks, of every query head of
 // the group, that see a tile of 128 keys (4 products a block).  One kernel
@@ -43,35 +43,138 @@ struct BwTile {
   static_assert(SMEM <= 227 * 1024, "shared memory of a block");
 };
 
+// P and dS are rounded to the operands' type for their products: the tensor
+// cores take two operands of one 16-bit type.  In bf16 that is 2^-8 of each
+// value, whatever its size.  fp16 has the range 2^-14 to 65504, and neither
+// keeps within it: P is 1 / n for n keys seen alike, and |dS| = P |dP - delta| <=
+// 2 N, N the norm of a dout row times the largest norm of a v row, is as large or
+// small as dout.  So in fp16 both are held times powers of two, taken out again
+// when dk, dv and dq are stored: P times 2^14, dS times 2^e with 2^e 2 N <= 2^15
+// (and above 2^14), e from the row's own norm in attn_dq and from the largest
+// in attn_dkv, where a sum runs over the rows.  What is lost then lies under N 2^-38.
+constexpr int BW_P_SHIFT = 14;
+template <typename T>
+struct Shifted {
+  static constexpr bool value = DtOf<T>::value == PKM_DT_F16;
+};
+__device__ __forceinline__ int ds_shift(float n) {  // e for N = n; 0 without a bound
+  return n > 0.f && n < INFINITY ? 13 - ((int)(__float_as_uint(n) >> 23) - 127) : 0;
+}
+__device__ __forceinline__ float power2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Raises *peak to the square root of the block's largest `square` (none is
+// infinite or NaN).  A maximum of non-negative numbers: the order of the updates
+// does not show.  One update a block, and only above what was there: an update
+// for every row took 30 us for 43000 rows.
+__device__ __forceinline__ void raise_peak(float* peak, float old, float square) {
+  __shared__ float squares[8];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) square = fmaxf(square, __shfl_xor_sync(~0u, square, o));
+  if ((threadIdx.x & 31) == 0) squares[threadIdx.x >> 5] = square;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) square = fmaxf(square, squares[i]);
+    square = sqrtf(square);
+    if (square > old) atomicMax(reinterpret_cast<int*>(peak), __float_as_int(square));
+  }
+}
+
 // ---------------------------------------------------------------------------
-// delta = sum over the channels of dout * (out + out_lo): 16 lanes a row, 16
-// bytes each.  (From out alone, rounded, a row with few visible keys had 1.7
-// times the rounding error of dq, and not 1.4 times.)
+// delta = sum over the channels of dout * (out + out_lo): a block takes 128 rows
+// of a head, 16 lanes a row, 16 bytes each, four rows in flight a thread.  (From
+// out alone, rounded, a row with few visible keys had 1.7 times the rounding error
+// of dq, and not 1.4 times.)
+// fp16: the norms of dout's rows too, and the largest of dout's and (the first
+// v_blocks blocks) of v's rows of each key/value head.
 // ---------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnBwdArgs g, FastDiv by_t, FastDiv by_h) {
+__global__ void __launch_bounds__(256)
+    attn_delta_kernel(const AttnBwdArgs g, FastDiv by_tiles, FastDiv by_h, FastDiv by_v_tiles, uint32_t v_blocks) {
   const AttnArgs& a = g.f;
-  const uint32_t r = blockIdx.x * 16u + (threadIdx.x >> 4);
-  const uint32_t bh = by_t.div(r), t = r - bh * a.Tq;
-  if (bh >= (uint32_t)a.B * a.Hq) return;  // (whole rows of lanes leave)
-  const uint32_t b = by_h.div(bh), h = bh - b * a.Hq;
-  const int d = (threadIdx.x & 15) * 8;
-  float sum = 0.f;
-  if (d < a.D) {
-    float u[8], lo[8], v[8];
-    const int64_t at = b * a.so.b + h * a.so.h + (int64_t)t * a.so.t + d;
-    VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + at), u);
-    VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_lo) + at), lo);
-    VecTraits<T>::unpack(*reinterpret_cast<const uint4*>(static_cast<const T*>(g.dout) + b * g.sdo.b + h * g.sdo.h +
-                                                         (int64_t)t * g.sdo.t + d),
-                         v);
+  const int d = (threadIdx.x & 15) * 8, rl = threadIdx.x >> 4;
+  const bool in = d < a.D;
+  constexpr int R = 4;  // rows in flight
+  constexpr uint4 zero = {0, 0, 0, 0};
+  if (Shifted<T>::value && blockIdx.x < v_blocks) {
+    const uint32_t bh = by_v_tiles.div(blockIdx.x);
+    const int b = bh / a.Hk, hk = bh % a.Hk, row = (int)(blockIdx.x - bh * by_v_tiles.d) * AT_T + rl;
+    const Span sp = attn_span(a.starts, a.ends, b, a.Tk);
+    const T* v = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + d;
+    float* peak = g.peaks + ((int64_t)a.B * a.Hk + bh) * AT_PEAK;
+    const float old = __ldcg(peak);
+    float largest = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < AT_T; i += 16 * R) {
+      uint4 x[R];
 #pragma unroll
-    for (int y = 0; y < 8; ++y) sum = fmaf(u[y] + lo[y], v[y], sum);
+      for (int y = 0; y < R; ++y) {
+        const int t = row + i + 16 * y;
+        x[y] = in && t >= sp.start && t < sp.end ? *reinterpret_cast<const uint4*>(v + t * a.sv.t) : zero;
+      }
+#pragma unroll
+      for (int y = 0; y < R; ++y) {
+        float u[8], square = 0.f;
+        VecTraits<T>::unpack(x[y], u);
+#pragma unroll
+        for (int z = 0; z < 8; ++z) square = fmaf(u[z], u[z], square);
+#pragma unroll
+        for (int o = 8; o; o >>= 1) square += __shfl_xor_sync(~0u, square, o);
+        if (square < INFINITY) largest = fmaxf(largest, square);
+      }
+    }
+    raise_peak(peak, old, largest);
+    return;
   }
-  const uint32_t row = 0xffffu << (threadIdx.x & 16);
+  const uint32_t item = blockIdx.x - v_blocks, bh = by_tiles.div(item), b = by_h.div(bh), h = bh - b * a.Hq;
+  const int row = (int)(item - bh * by_tiles.d) * AT_T + rl;
+  const T* out = static_cast<const T*>(a.out) + b * a.so.b + h * a.so.h + d;
+  const T* out_lo = static_cast<const T*>(a.out_lo) + b * a.so.b + h * a.so.h + d;
+  const T* dout = static_cast<const T*>(g.dout) + b * g.sdo.b + h * g.sdo.h + d;
+  float* peak = nullptr;
+  float old = 0.f, largest = 0.f;
+  Span sp{};
+  if (Shifted<T>::value) {
+    peak = g.peaks + ((int64_t)b * a.Hk + h / a.G) * AT_PEAK;
+    old = __ldcg(peak);
+    sp = attn_span(a.starts, a.ends, (int)b, a.Tk);
+  }
+#pragma unroll 1
+  for (int i = 0; i < AT_T; i += 16 * R) {
+    uint4 x[R], lo[R], y[R];
 #pragma unroll
-  for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(row, sum, o);
-  if ((threadIdx.x & 15) == 0) g.delta[r] = sum;
+    for (int z = 0; z < R; ++z) {
+      const int t = row + i + 16 * z;
+      const bool ok = in && t < a.Tq;
+      x[z] = ok ? *reinterpret_cast<const uint4*>(out + t * a.so.t) : zero;
+      lo[z] = ok ? *reinterpret_cast<const uint4*>(out_lo + t * a.so.t) : zero;
+      y[z] = ok ? *reinterpret_cast<const uint4*>(dout + t * g.sdo.t) : zero;
+    }
+#pragma unroll
+    for (int z = 0; z < R; ++z) {
+      float u[8], l[8], v[8], sum = 0.f, square = 0.f;
+      VecTraits<T>::unpack(x[z], u);
+      VecTraits<T>::unpack(lo[z], l);
+      VecTraits<T>::unpack(y[z], v);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        sum = fmaf(u[c] + l[c], v[c], sum);
+        if (Shifted<T>::value) square = fmaf(v[c], v[c], square);
+      }
+#pragma unroll
+      for (int o = 8; o; o >>= 1) {
+        sum += __shfl_xor_sync(~0u, sum, o);
+        if (Shifted<T>::value) square += __shfl_xor_sync(~0u, square, o);
+      }
+      const int t = row + i + 16 * z;
+      if ((threadIdx.x & 15) == 0 && t < a.Tq) g.delta[(int64_t)bh * a.Tq + t] = sum;
+      if (Shifted<T>::value && t < a.Tq) {
+        if ((threadIdx.x & 15) == 0) g.norms[(int64_t)bh * a.Tq + t] = sqrtf(square);
+        const int p = t + a.Tk - a.Tq;
+        if (p >= sp.start && p < sp.end && square < INFINITY) largest = fmaxf(largest, square);
+      }
+    }
+  }
+  if (Shifted<T>::value) raise_peak(peak, old, largest);
 }
 
 // ---------------------------------------------------------------------------
@@ -325,11 +428,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const int row = w.r0 + rl, pr = row + w.shift;
       const bool real = row < a.Tq && pr >= 0 && pr < w.len;
       const int first = w.r0 + w.shift, last = first + AT_T - 1;
-      float delta = 0.f, lse = 0.f;
+      float delta = 0.f, lse = 0.f, f = a.scale;  // f: dq is stored times it
       if (real) {
         const int64_t stat = ((int64_t)w.b * a.Hq + w.h) * a.Tq + row;
         delta = g.delta[stat];
         lse = a.lse[stat] * AT_LOG2E;
+        if (Shifted<T>::value) {
+          const int e = ds_shift(g.norms[stat] * g.peaks[((int64_t)(a.B + w.b) * a.Hk + w.hk) * AT_PEAK]);
+          lse -= e;
+          f *= power2(-e);
+        }
       }
       for (int n = 0; n < walk.count; ++n, ++nb) {
         ok = at_wait(&s_full[nb & 1], (nb >> 1) & 1, a.err, abort_flag);
@@ -377,10 +485,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       if (!(ok = named_all(1 + half, ok))) break;
       // each half of the threads stores 64 of the channels (the first all of them where there are no more)
       if (DP == 128)
-        store_tile<T, 64>(t_dq + lanes + half * 64, so + half * AT_BOX, rl, a.scale, real, walk.count > 0, &tdq, w.r0,
+        store_tile<T, 64>(t_dq + lanes + half * 64, so + half * AT_BOX, rl, f, real, walk.count > 0, &tdq, w.r0,
                           w.h, w.b, 1 + half, leader, o_empty, half * 64);
       else if (half == 0)
-        store_tile<T, 64>(t_dq + lanes, so, rl, a.scale, real, walk.count > 0, &tdq, w.r0, w.h, w.b, 1, leader,
+        store_tile<T, 64>(t_dq + lanes, so, rl, f, real, walk.count > 0, &tdq, w.r0, w.h, w.b, 1, leader,
                           o_empty);
       else if (walk.count > 0)
         mbar_arrive(o_empty);
@@ -449,6 +557,12 @@ struct DkvItem {
     tail = nq > 0 ? i_end - (i_base + (n0 + nq - 1) * AT_T) : AT_T;  // queries in a head's last block
   }
 };
+
+// e of attn_dkv, one for a key/value head.
+__device__ __forceinline__ int dkv_shift(const AttnBwdArgs& g, int b, int hk) {
+  const float* p = g.peaks + ((int64_t)b * g.f.Hk + hk) * AT_PEAK;
+  return ds_shift(p[0] * p[(int64_t)g.f.B * g.f.Hk * AT_PEAK]);
+}
 
 // Rows of TMEM are keys.  TMEM: S^T (columns 0; P^T over it, the halves of
 // the block's queries at 0 and 64), dP^T (128; dS^T over it), dv (256), dk
@@ -665,6 +779,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     bool ok = true;
     while (ok && items.next(item)) {
       const DkvItem w(g, item);
+      // lse less P's shift, delta times what is left of dS's
+      constexpr float PS = Shifted<T>::value ? BW_P_SHIFT : 0;
+      const float ds = Shifted<T>::value && w.count > 0 ? power2(dkv_shift(g, w.b, w.hk) - BW_P_SHIFT) : 1.f;
       int h = w.hk * a.G, q = 0;
       for (int n = 0; n < w.count; ++n, ++nb) {
         const int st = nb % ST;
@@ -676,8 +793,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         for (int x = 0; x < 4; ++x) {
           const int r = row + x * 32 + lane;
           const bool in = r < w.i_end;
-          rows[(st * 2) * AT_T + x * 32 + lane] = in ? a.lse[base + r] * AT_LOG2E : 0.f;
-          rows[(st * 2 + 1) * AT_T + x * 32 + lane] = in ? g.delta[base + r] : 0.f;
+          rows[(st * 2) * AT_T + x * 32 + lane] = in ? a.lse[base + r] * AT_LOG2E - PS : 0.f;
+          rows[(st * 2 + 1) * AT_T + x * 32 + lane] = in ? g.delta[base + r] * ds : 0.f;
         }
         mbar_arrive(&l_full[st]);
         if (++q == w.nq) {
@@ -720,6 +837,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const DkvItem w(g, item);
       const int jr = w.j0 + rl - w.start;
       const bool real = w.j0 + rl < a.Tk && jr >= 0 && jr < w.len;
+      const int e = Shifted<T>::value && w.count > 0 ? dkv_shift(g, w.b, w.hk) : 0;
+      const float ds = power2(e - BW_P_SHIFT);  // (fp16)
       int q = 0;
       for (int n = 0; n < w.count; ++n, ++nb) {
         const int st = nb % ST;
@@ -772,10 +891,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         tmem_ld_wait();
 #pragma unroll
         for (int y = 0; y < 64; y += 4) {
-          const float4 e = lds_f4(delta + y * 4);
-          v[y / 2] = pack2<T>(p[y] * (__uint_as_float(d[y]) - e.x), p[y + 1] * (__uint_as_float(d[y + 1]) - e.y));
-          v[y / 2 + 1] =
-              pack2<T>(p[y + 2] * (__uint_as_float(d[y + 2]) - e.z), p[y + 3] * (__uint_as_float(d[y + 3]) - e.w));
+          const float4 m = lds_f4(delta + y * 4);
+          auto diff = [&](uint32_t dp, float m) {
+            return Shifted<T>::value ? fmaf(__uint_as_float(dp), ds, -m) : __uint_as_float(dp) - m;
+          };
+          v[y / 2] = pack2<T>(p[y] * diff(d[y], m.x), p[y + 1] * diff(d[y + 1], m.y));
+          v[y / 2 + 1] = pack2<T>(p[y + 2] * diff(d[y + 2], m.z), p[y + 3] * diff(d[y + 3], m.w));
         }
         mbar_arrive(&l_empty[st]);
         tmem_st_32x32b_x32(td, v);
@@ -791,7 +912,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       if (!(ok = named_all(1 + half, ok))) break;
       // the first half of the threads stores dv, the second dk
       const uint32_t acc = (half ? t_dk : t_dv) + lanes;
-      const float f = half ? a.scale : 1.f;
+      const float f = !Shifted<T>::value ? (half ? a.scale : 1.f) : half ? a.scale * power2(-e) : power2(-BW_P_SHIFT);
       if (FAR && w.slot >= 0)
         store_part<DP>(acc, so + half * AT_BOX, rl, f, real, w.count > 0, half ? &tpk : &tpv, a.D, 0, 0, w.slot,
                        1 + half, leader, acc_empty);
@@ -891,8 +1012,13 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
     return fail(PKM_ERR_UNSUPPORTED, "too many rows");
   const int sms = num_sms();
   if (rows > 0) {
-    attn_delta_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(g, FastDiv((uint32_t)a.Tq),
-                                                                       FastDiv((uint32_t)a.Hq));
+    const int64_t tiles = (a.Tq + AT_T - 1) / AT_T, v_tiles = (a.Tk + AT_T - 1) / AT_T;
+    const int64_t v_blocks = Shifted<T>::value ? v_tiles * a.B * a.Hk : 0;
+    if (v_blocks &&
+        cudaMemsetAsync(g.peaks, 0, (size_t)a.B * a.Hk * 2 * AT_PEAK * sizeof(float), st) != cudaSuccess)
+      return check_cuda("cudaMemsetAsync(attn_bwd)");
+    attn_delta_kernel<T><<<(unsigned)(tiles * a.B * a.Hq + v_blocks), 256, 0, st>>>(
+        g, FastDiv((uint32_t)tiles), FastDiv((uint32_t)a.Hq), FastDiv((uint32_t)v_tiles), (uint32_t)v_blocks);
     attn_dq_kernel<T, DP><<<(unsigned)std::min<int64_t>(gq, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdq, g);
   }
   if ((rc = check_cuda("attn_dq"))) return rc;
