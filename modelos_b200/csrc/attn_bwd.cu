@@ -963,16 +963,20 @@ __global__ void __launch_bounds__(256) attn_far_join_kernel(const AttnBwdArgs g,
 // Items for the queries behind a sink's window pay where such a tile's walk
 // over all queries is more than half of what a multiprocessor has to do: 1187
 // tokens x 3, 12/4 heads: dk and dv 56 -> 40 us; but 2048 x 8, 16/8 heads, where
-// it is a third: 183 -> 206.
+// it is a third: 183 -> 206.  Many sinks are many such walks, which fill the GPU
+// by themselves; and there are only as many parts as make two items a
+// multiprocessor.  So the parts' sums take at most 12 * 128 rows of dk and dv for
+// each multiprocessor (233 MB for heads of 128), whatever the sizes.
 size_t attn_bwd_far(AttnBwdArgs& g) {
   const AttnArgs& a = g.f;
   g.far_tiles = g.far_parts = 0;
   if (!a.window || !a.sinks || !a.Tq) return 0;
   const int64_t heads = (int64_t)a.B * a.Hk, tiles = (a.Tk + AT_T - 1) / AT_T;
   const int64_t all = (a.Tq + AT_T - 1) / AT_T + 1, near = (a.window + AT_T - 1) / AT_T + 2;
-  if (all < 2 * near || 2 * all * num_sms() < heads * (tiles * near + all)) return 0;
-  g.far_tiles = (a.sinks - 1) / AT_T + 2;
-  g.far_parts = (int)std::min<int64_t>(16, (all - 1) / near);
+  const int64_t walks = (a.sinks - 1) / AT_T + 1, slots = 2 * num_sms();
+  if (all < 2 * near || all * slots < heads * (tiles * near + walks * all)) return 0;
+  g.far_tiles = (int)walks + 1;  // (they may begin inside a tile)
+  g.far_parts = (int)std::min<int64_t>({16, (all - 1) / near, (slots + heads * walks - 1) / (heads * walks)});
   return (size_t)heads * g.far_tiles * (g.far_parts + 1) * AT_T * a.D * 2 * sizeof(float);
 }
 
