@@ -243,12 +243,12 @@ def check_device_errors(dev: Optional[torch.device] = None):
     v = read_device_errors(dev)
     if v & DEVERR_INDEX:
         raise IndexError("modelos_b200: an embedding index was outside [0, num_rows)")
+    if v & DEVERR_TIMEOUT:
+        raise RuntimeError("modelos_b200: a bounded wait inside a kernel timed out")
     if v & DEVERR_CAPACITY:
         raise IndexError("modelos_b200: a token's row was outside the 4-bit cache")
     if v & DEVERR_MASK:
         raise ValueError(MASK_HOLES)
-    if v & DEVERR_TIMEOUT:
-        raise RuntimeError("modelos_b200: a bounded wait inside a kernel timed out")
 
 
 # ---------------------------------------------------------------------------
