@@ -380,7 +380,12 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
             }
           }
         }
-        uint32_t pb[F::SUB][NT][2];
+        // Probabilities in the keys' type for the product.  16 bits: with what
+        // their rounding left as a second product, which the time, the copies',
+        // does not show; without it the output's error was 1.4 times that of its
+        // own rounding.  4 bits: the kernel is bound by instructions, and the
+        // codes' error is many times larger.
+        uint32_t pb[F::SUB][NT][2], pl[F::SUB][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float ma = m[nt][0] == -INFINITY ? 0.f : m[nt][0], mb = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
@@ -390,8 +395,16 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
             const float p2 = ex2(x[sub][nt][2] - ma), p3 = ex2(x[sub][nt][3] - mb);
             l[nt][0] += p0 + p2;
             l[nt][1] += p1 + p3;
-            pb[sub][nt][0] = transpose8x8(pack2<T>(p0, p1));
-            pb[sub][nt][1] = transpose8x8(pack2<T>(p2, p3));
+            const uint32_t h0 = pack2<T>(p0, p1), h1 = pack2<T>(p2, p3);
+            pb[sub][nt][0] = transpose8x8(h0);
+            pb[sub][nt][1] = transpose8x8(h1);
+            if constexpr (!Q4) {
+              float f[2];
+              unpack2<T>(h0, f);
+              pl[sub][nt][0] = transpose8x8(pack2<T>(p0 - f[0], p1 - f[1]));
+              unpack2<T>(h1, f);
+              pl[sub][nt][1] = transpose8x8(pack2<T>(p2 - f[0], p3 - f[1]));
+            }
           }
         }
         // ---- O^T += V^T P^T; keys behind the stage's count may hold anything
@@ -454,7 +467,10 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
                 r[3] &= keep1;
               }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][s], r, pb[sub][nt][0], pb[sub][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<T>(o[nt][s], r, pb[sub][nt][0], pb[sub][nt][1]);
+                mma16816<T>(o[nt][s], r, pl[sub][nt][0], pl[sub][nt][1]);
+              }
             }
           }
         }
