@@ -86,6 +86,8 @@ int attn_fwd_launch(const AttnArgs& a, int dtype, void* workspace, cudaStream_t 
 // item's keys in the other.
 bool attn_few_rows(int64_t B, int64_t Hk, int64_t G, int64_t Tq);
 int attn_fwd_splits(int64_t B, int64_t Hk, int64_t G, int64_t Tq, int64_t Tk, int64_t window, int64_t sinks);
+// Whether P and dS take part in their products with their rounding's remainders.
+bool attn_exact(const AttnArgs& a);
 // Sets far_tiles and far_parts; returns the bytes their partial sums take.
 size_t attn_bwd_far(AttnBwdArgs& g);
 int attn_bwd_launch(const AttnBwdArgs& g, int dtype, void* partials, cudaStream_t st);

@@ -205,7 +205,9 @@ struct DqItem {
 
 // TMEM: S in two buffers (columns 0, 128), dP (256; dS over it: the halves of
 // the block's columns at 256 and 320), dq (384).
-template <typename T, int DP>
+// EXACT: a second product adds what rounding dS left, which lies behind each half
+// of dS.
+template <typename T, int DP, bool EXACT>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dq_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo,
                    const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -384,6 +386,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           tc_fence_after();
           if (elect_one()) {
             at_accum<64>(to, tp, km + (nb % ST) * STEP, ID_O, n == 0);  // dq += dS K
+            if (EXACT) at_accum<64>(to, tp + 32, km + (nb % ST) * STEP, ID_O, false);
             umma_commit(&k_empty[nb % ST]);
             if (!more) umma_commit(o_full);
           }
@@ -464,15 +467,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         ok = at_wait(dp_full, nb & 1, a.err, abort_flag);
         if (!(ok = __all_sync(~0u, ok))) break;
         tc_fence_after();
-        uint32_t d[64], ds[32];
+        uint32_t d[64], ds[32], lo[EXACT ? 32 : 1];
         tmem_ld_32x32b_x32(t_dp + lanes + half * 64, reinterpret_cast<uint32_t(&)[32]>(d[0]));
         tmem_ld_32x32b_x32(t_dp + lanes + half * 64 + 32, reinterpret_cast<uint32_t(&)[32]>(d[32]));
         tmem_ld_wait();
 #pragma unroll
-        for (int y = 0; y < 32; ++y)
-          ds[y] = pack2<T>(p[2 * y] * (__uint_as_float(d[2 * y]) - delta),
-                           p[2 * y + 1] * (__uint_as_float(d[2 * y + 1]) - delta));
+        for (int y = 0; y < 32; ++y) {
+          const float x0 = p[2 * y] * (__uint_as_float(d[2 * y]) - delta);
+          const float x1 = p[2 * y + 1] * (__uint_as_float(d[2 * y + 1]) - delta);
+          ds[y] = pack2<T>(x0, x1);
+          if constexpr (EXACT) lo[y] = remainder2<T>(x0, x1, ds[y]);
+        }
         tmem_st_32x32b_x32(t_dp + lanes + half * 64, ds);
+        if constexpr (EXACT) tmem_st_32x32b_x32(t_dp + lanes + half * 64 + 32, lo);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(ds_full);
@@ -568,8 +575,10 @@ __device__ __forceinline__ int dkv_shift(const AttnBwdArgs& g, int b, int hk) {
 // the block's queries at 0 and 64), dP^T (128; dS^T over it), dv (256), dk
 // (256 + DP).
 // FAR: some items are parts, stored in 32 bits (compiled apart: with both ways to
-// store in one kernel the compiler spills registers).
-template <typename T, int DP, bool FAR>
+// store in one kernel the compiler spills registers).  EXACT: second products add
+// what rounding P and dS left, which lies behind each half of them.
+enum DkvMode { DKV_PLAIN, DKV_FAR, DKV_EXACT };
+template <typename T, int DP, DkvMode MODE>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dkv_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tdo,
                     const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -578,6 +587,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     const AttnBwdArgs g) {
   const AttnArgs& a = g.f;
   using F = BwTile<DP>;
+  constexpr bool FAR = MODE == DKV_FAR, EXACT = MODE == DKV_EXACT;
   constexpr int ST = F::STAGES;
   constexpr int FMT = DtOf<T>::value == PKM_DT_BF16 ? 1 : 0;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -751,6 +761,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           tc_fence_after();
           if (elect_one()) {
             at_accum<64>(uv, us, dm + st * STEP, ID_O, n == 0);  // dv += P^T dout
+            if (EXACT) at_accum<64>(uv, us + 32, dm + st * STEP, ID_O, false);
             umma_commit(&o_empty[st]);
           }
           __syncwarp();
@@ -759,6 +770,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           tc_fence_after();
           if (elect_one()) {
             at_accum<64>(uk, up, qm + st * STEP, ID_O, n == 0);  // dk += dS^T Q
+            if (EXACT) at_accum<64>(uk, up + 32, qm + st * STEP, ID_O, false);
             umma_commit(&q_empty[st]);
             if (!more) umma_commit(done);
           }
@@ -879,6 +891,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
         for (int x = 0; x < 32; ++x) v[x] = pack2<T>(p[2 * x], p[2 * x + 1]);
         tmem_st_32x32b_x32(ts, v);
+        if constexpr (EXACT) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) v[x] = remainder2<T>(p[2 * x], p[2 * x + 1], v[x]);
+          tmem_st_32x32b_x32(ts + 32, v);
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_full);
@@ -895,11 +912,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           auto diff = [&](uint32_t dp, float m) {
             return Shifted<T>::value ? fmaf(__uint_as_float(dp), ds, -m) : __uint_as_float(dp) - m;
           };
-          v[y / 2] = pack2<T>(p[y] * diff(d[y], m.x), p[y + 1] * diff(d[y + 1], m.y));
-          v[y / 2 + 1] = pack2<T>(p[y + 2] * diff(d[y + 2], m.z), p[y + 3] * diff(d[y + 3], m.w));
+          p[y] *= diff(d[y], m.x);
+          p[y + 1] *= diff(d[y + 1], m.y);
+          p[y + 2] *= diff(d[y + 2], m.z);
+          p[y + 3] *= diff(d[y + 3], m.w);
+          v[y / 2] = pack2<T>(p[y], p[y + 1]);
+          v[y / 2 + 1] = pack2<T>(p[y + 2], p[y + 3]);
         }
         mbar_arrive(&l_empty[st]);
         tmem_st_32x32b_x32(td, v);
+        if constexpr (EXACT) {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) v[x] = remainder2<T>(p[2 * x], p[2 * x + 1], v[x]);
+          tmem_st_32x32b_x32(td + 32, v);
+        }
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(ds_full);
@@ -970,7 +996,7 @@ __global__ void __launch_bounds__(256) attn_far_join_kernel(const AttnBwdArgs g,
 size_t attn_bwd_far(AttnBwdArgs& g) {
   const AttnArgs& a = g.f;
   g.far_tiles = g.far_parts = 0;
-  if (!a.window || !a.sinks || !a.Tq) return 0;
+  if (!a.window || !a.sinks || !a.Tq || attn_exact(a)) return 0;
   const int64_t heads = (int64_t)a.B * a.Hk, tiles = (a.Tk + AT_T - 1) / AT_T;
   const int64_t all = (a.Tq + AT_T - 1) / AT_T + 1, near = (a.window + AT_T - 1) / AT_T + 2;
   const int64_t walks = (a.sinks - 1) / AT_T + 1, slots = 2 * num_sms();
@@ -986,8 +1012,12 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
   constexpr int dt = DtOf<T>::value;
   constexpr int smem = BwTile<DP>::SMEM;
   // (before the tensor maps: it makes the device's context current on this thread)
-  const auto dkv = g.far_tiles ? attn_dkv_kernel<T, DP, true> : attn_dkv_kernel<T, DP, false>;
-  if (cudaFuncSetAttribute(attn_dq_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+  const bool exact = attn_exact(a);
+  const auto dq = exact ? attn_dq_kernel<T, DP, true> : attn_dq_kernel<T, DP, false>;
+  const auto dkv = g.far_tiles ? attn_dkv_kernel<T, DP, DKV_FAR>
+                   : exact     ? attn_dkv_kernel<T, DP, DKV_EXACT>
+                               : attn_dkv_kernel<T, DP, DKV_PLAIN>;
+  if (cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
       cudaFuncSetAttribute(dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return check_cuda("cudaFuncSetAttribute(attn_bwd)");
   CUtensorMap tq{}, tdo{}, tk, tv, tdq{}, tdk, tdv, tp[2]{};
@@ -1023,7 +1053,7 @@ static int attn_bwd_go(const AttnBwdArgs& g, void* partials, cudaStream_t st) {
       return check_cuda("cudaMemsetAsync(attn_bwd)");
     attn_delta_kernel<T><<<(unsigned)(tiles * a.B * a.Hq + v_blocks), 256, 0, st>>>(
         g, FastDiv((uint32_t)tiles), FastDiv((uint32_t)a.Hq), FastDiv((uint32_t)v_tiles), (uint32_t)v_blocks);
-    attn_dq_kernel<T, DP><<<(unsigned)std::min<int64_t>(gq, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdq, g);
+    dq<<<(unsigned)std::min<int64_t>(gq, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdq, g);
   }
   if ((rc = check_cuda("attn_dq"))) return rc;
   dkv<<<(unsigned)std::min<int64_t>(gk, sms), BW_THREADS, smem, st>>>(tq, tdo, tk, tv, tdk, tdv, tp[0], tp[1], g);

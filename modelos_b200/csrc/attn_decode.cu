@@ -399,11 +399,8 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
             pb[sub][nt][0] = transpose8x8(h0);
             pb[sub][nt][1] = transpose8x8(h1);
             if constexpr (!Q4) {
-              float f[2];
-              unpack2<T>(h0, f);
-              pl[sub][nt][0] = transpose8x8(pack2<T>(p0 - f[0], p1 - f[1]));
-              unpack2<T>(h1, f);
-              pl[sub][nt][1] = transpose8x8(pack2<T>(p2 - f[0], p3 - f[1]));
+              pl[sub][nt][0] = transpose8x8(remainder2<T>(p0, p1, h0));
+              pl[sub][nt][1] = transpose8x8(remainder2<T>(p2, p3, h1));
             }
           }
         }

@@ -99,13 +99,17 @@ struct FwItem {
 };
 
 // PART: items are parts of a split, stored in 32 bits (compiled apart: with both
-// ways to store in one kernel the compiler spills registers).
-template <typename T, int DP, bool PART>
+// ways to store in one kernel the compiler spills registers).  EXACT: a second
+// product adds what rounding the probabilities left; they lie behind P, over the
+// second half of S_i.
+enum FwMode { FW_PLAIN, FW_PART, FW_EXACT };
+template <typename T, int DP, FwMode MODE>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                     const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tout,
                     const __grid_constant__ CUtensorMap tlo, const AttnArgs a) {
   using F = FwTile<DP>;
+  constexpr bool PART = MODE == FW_PART, EXACT = MODE == FW_EXACT;
   constexpr int ST = F::STAGES;
   constexpr int FMT = DtOf<T>::value == PKM_DT_BF16 ? 1 : 0;
   extern __shared__ unsigned char smem_raw[];
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             tc_fence_after();
             if (elect_one()) {
               at_accum<32>(to + i * DP, ts + i * AT_T, v0 + st * STEP, ID_O, n == 0);  // O_i += P_i V(n)
+              if (EXACT) at_accum<32>(to + i * DP, ts + i * AT_T + 64, v0 + st * STEP, ID_O, false);
               if (i == w.nt - 1) umma_commit(&v_empty[st]);
               if (more) {  // S_i = Q_i K(n + 1)^T
                 at_scores<DP>(ts + i * AT_T, q0 + i * STEP, k0 + nx * STEP, ID_S);
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          uint32_t p[32];
+          uint32_t p[32], lo[EXACT ? 32 : 1];
 #pragma unroll
           for (int y = 0; y < 32; ++y) {
             const float p0 = ex2(fmaf(__uint_as_float(s[x * 64 + 2 * y]), c, -mm));
@@ -407,8 +412,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             l4[2 * (y & 1)] += p0;
             l4[2 * (y & 1) + 1] += p1;
             p[y] = pack2<T>(p0, p1);
+            if constexpr (EXACT) lo[y] = remainder2<T>(p0, p1, p[y]);
           }
           tmem_st_32x32b_x32(ts + x * 32, p);
+          if constexpr (EXACT) tmem_st_32x32b_x32(ts + 64 + x * 32, lo);
         }
         l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
         tmem_st_wait();
@@ -529,8 +536,24 @@ int attn_fwd_splits(int64_t B, int64_t Hk, int64_t G, int64_t Tq, int64_t Tk, in
   return (int)std::max<int64_t>(1, std::min<int64_t>({num_sms() / std::max<int64_t>(items, 1), keys / (4 * AT_T), 16}));
 }
 
-template <typename T, int DP, bool PART>
+// Probabilities and their gradients are rounded to the operands' type for the
+// products, u of each value, in effect at random: outputs and gradients are off
+// by 1.2 to 1.5 times their own rounding (the most where a row sees few keys, and
+// where few rows leave the sum to chance).  A second product with the remainders
+// costs a fifth of a large call; where at most one tile a multiprocessor walks
+// few blocks, launches are what a call takes and it does not show (2 heads of 32,
+// 2 x 24 tokens: 87 us a training step's calls with and without), so there it is made.
+bool attn_exact(const AttnArgs& a) {
+  const int64_t tiles = (a.Tq + AT_T - 1) / AT_T, rows = tiles * a.G;
+  int64_t blocks = (a.Tk + AT_T - 1) / AT_T;
+  if (a.window)
+    blocks = std::min<int64_t>(blocks, (a.window + AT_T - 2) / AT_T + 1 + (a.sinks + AT_T - 1) / AT_T);
+  return blocks <= 4 && rows <= 9 && rows * a.B * a.Hk <= num_sms();
+}
+
+template <typename T, int DP, FwMode MODE>
 static int attn_fwd_go(const AttnArgs& a0, void* workspace, cudaStream_t st) {
+  constexpr bool PART = MODE == FW_PART;
   AttnArgs a = a0;
   JoinArgs join{};
   Strides3 so = a.so;
@@ -547,7 +570,7 @@ static int attn_fwd_go(const AttnArgs& a0, void* workspace, cudaStream_t st) {
   constexpr int dt = DtOf<T>::value;
   // (also makes the device's context current: a tensor map cannot be encoded
   // on a thread that has made no CUDA call yet, such as autograd's)
-  if (cudaFuncSetAttribute(attn_fwd_kernel<T, DP, PART>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(attn_fwd_kernel<T, DP, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            FwTile<DP>::SMEM) != cudaSuccess)
     return check_cuda("cudaFuncSetAttribute(attn_fwd)");
   CUtensorMap tq, tk, tv, tout, tlo{};
@@ -562,7 +585,7 @@ static int attn_fwd_go(const AttnArgs& a0, void* workspace, cudaStream_t st) {
   const int64_t items = (tiles + 1) / 2 * a.B * a.Hk * a.splits;
   if (items > INT32_MAX / 2) return fail(PKM_ERR_UNSUPPORTED, "too many rows");
   const int grid = (int)std::min<int64_t>(items, num_sms());
-  attn_fwd_kernel<T, DP, PART><<<grid, FW_THREADS, FwTile<DP>::SMEM, st>>>(tq, tk, tv, tout, tlo, a);
+  attn_fwd_kernel<T, DP, MODE><<<grid, FW_THREADS, FwTile<DP>::SMEM, st>>>(tq, tk, tv, tout, tlo, a);
   if ((rc = check_cuda("attn_fwd")) || !PART) return rc;
   attn_join_kernel<T><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(join, FastDiv((uint32_t)a.Tq),
                                                                    FastDiv((uint32_t)a.Hq));
@@ -571,7 +594,9 @@ static int attn_fwd_go(const AttnArgs& a0, void* workspace, cudaStream_t st) {
 
 template <typename T, int DP>
 static int attn_fwd_parts(const AttnArgs& a, void* workspace, cudaStream_t st) {
-  return a.splits > 1 ? attn_fwd_go<T, DP, true>(a, workspace, st) : attn_fwd_go<T, DP, false>(a, workspace, st);
+  return a.splits > 1    ? attn_fwd_go<T, DP, FW_PART>(a, workspace, st)
+         : attn_exact(a) ? attn_fwd_go<T, DP, FW_EXACT>(a, workspace, st)
+                         : attn_fwd_go<T, DP, FW_PLAIN>(a, workspace, st);
 }
 
 int attn_fwd_launch(const AttnArgs& a, int dtype, void* workspace, cudaStream_t st) {

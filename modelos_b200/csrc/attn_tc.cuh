@@ -137,6 +137,14 @@ __device__ __forceinline__ void unpack2<__half>(uint32_t w, float (&f)[2]) {
   f[1] = t.y;
 }
 
+// What packing (x, y) to w left, packed.
+template <typename T>
+__device__ __forceinline__ uint32_t remainder2(float x, float y, uint32_t w) {
+  float f[2];
+  unpack2<T>(w, f);
+  return pack2<T>(x - f[0], y - f[1]);
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
