@@ -537,18 +537,18 @@ int attn_fwd_splits(int64_t B, int64_t Hk, int64_t G, int64_t Tq, int64_t Tk, in
 }
 
 // Probabilities and their gradients are rounded to the operands' type for the
-// products, u of each value, in effect at random: outputs and gradients are off
-// by 1.2 to 1.5 times their own rounding (the most where a row sees few keys, and
-// where few rows leave the sum to chance).  A second product with the remainders
-// costs a fifth of a large call; where at most one tile a multiprocessor walks
-// few blocks, launches are what a call takes and it does not show (2 heads of 32,
-// 2 x 24 tokens: 87 us a training step's calls with and without), so there it is made.
+// products, u of each value, in effect at random: outputs and gradients are off by
+// 1.2 to 1.5 times their own rounding, the most where a row sees few keys, and 1.65
+// times where few rows leave the sum to chance as well.  A second product with
+// the remainders makes that 1.00, for a third of the time (8192 tokens, forward and
+// backward, 1.01 -> 1.32 ms; up to 512 tokens, 55 -> 65 us).  So it is made where few
+// keys are seen and at most one tile falls to a multiprocessor, a call bound by
+// launches (9 x 128 tokens, 16/8 heads: 37 -> 39 us of kernels, 92 us the call;
+// 2 x 24 tokens, 2/1 heads of 32: 26.5 -> 29.8).
 bool attn_exact(const AttnArgs& a) {
-  const int64_t tiles = (a.Tq + AT_T - 1) / AT_T, rows = tiles * a.G;
-  int64_t blocks = (a.Tk + AT_T - 1) / AT_T;
-  if (a.window)
-    blocks = std::min<int64_t>(blocks, (a.window + AT_T - 2) / AT_T + 1 + (a.sinks + AT_T - 1) / AT_T);
-  return blocks <= 4 && rows <= 9 && rows * a.B * a.Hk <= num_sms();
+  const int64_t rows = (int64_t)((a.Tq + AT_T - 1) / AT_T) * a.G;
+  const bool few = a.Tk <= AT_T || (a.window && a.window + a.sinks <= 32);
+  return few && rows <= 16 && rows * a.B * a.Hk <= num_sms();
 }
 
 template <typename T, int DP, FwMode MODE>

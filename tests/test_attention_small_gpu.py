@@ -1,4 +1,4 @@
-"""Small calls, bound by launches: outputs and gradients are off by their own
+"""Small calls over few keys, bound by launches: outputs and gradients are off by their own
 rounding, not by those of the probabilities and their gradients (which take part
 with their remainders)."""
 from __future__ import annotations
@@ -55,9 +55,11 @@ def bounds(q, k, v, dout, window, sinks, scale, starts, ends):
 
 
 @pytest.mark.parametrize("dtype,D", [(BF, 128), (BF, 64), (BF, 40), (HF, 64), (HF, 120)])
-@pytest.mark.parametrize("shape", [(2, 2, 1, 24, 24), (1, 2, 1, 17, 200), (2, 4, 2, 130, 130), (1, 6, 2, 200, 450),
-                                   (3, 3, 3, 290, 290)])
-@pytest.mark.parametrize("window,sinks,pad", [(0, 0, 0), (8, 2, 3), (100, 0, 7)])
+@pytest.mark.parametrize("shape,window,sinks,pad", [
+    (shape, *mask) for shape in ((2, 2, 1, 24, 24), (1, 2, 1, 17, 100), (2, 4, 2, 101, 101), (1, 6, 2, 60, 128),
+                                 (3, 3, 3, 128, 128))
+    for mask in ((0, 0, 0), (8, 2, 3), (100, 0, 7))
+] + [((1, 2, 1, 450, 600), 20, 4, 0), ((2, 4, 2, 300, 300), 1, 0, 5), ((2, 3, 1, 513, 513), 31, 1, 9)])
 def test_output_and_gradients(dtype, D, shape, window, sinks, pad):
     from modelos_b200 import _native
     from modelos_b200.attention import window_attention
