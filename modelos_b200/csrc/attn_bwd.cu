@@ -20,9 +20,9 @@
 // block before.
 //
 // Measured (16/8 heads of 128, bf16): 8192 tokens, all visible, dq 0.32 ms, dk
-// and dv 0.43 ms, delta 0.02: 900 TFLOP/s of the five products that the gradients
-// need, 1260 of the seven that run.  8 x 2048 tokens, window 512: 0.14, 0.19 and
-// 0.04 ms.
+// and dv 0.42 ms, delta 0.015: 910 TFLOP/s of the five products that the gradients
+// need, 1300 of the seven that run.  8 x 2048 tokens, window 512: 0.14, 0.18 and
+// 0.036 ms.
 #include <algorithm>
 
 #include "attn_tc.cuh"
@@ -44,7 +44,8 @@ struct BwTile {
 };
 
 // P and dS are rounded to the operands' type for their products: the tensor
-// cores take two operands of one 16-bit type.  In bf16 that is 2^-8 of each
+// cores take two operands of one 16-bit type (attn_exact() has what that costs in
+// accuracy and where it is avoided).  In bf16 that is 2^-8 of each
 // value, whatever its size.  fp16 has the range 2^-14 to 65504, and neither
 // keeps within it: P is 1 / n for n keys seen alike, and |dS| = P |dP - delta| <=
 // 2 N, N the norm of a dout row times the largest norm of a v row, is as large or

@@ -7,8 +7,10 @@
 // products run while the last one's output is stored.
 //   warps 0-3, 4-7  softmax of tile 0, 1: a thread owns a row; it reads its
 //                   128 scores from TMEM, writes the probabilities back over
-//                   them in the operands' type, and keeps maximum and sum in
-//                   registers;
+//                   them in the operands' type (the tensor cores take two
+//                   operands of one 16-bit type; attn_exact() has what that
+//                   costs in accuracy and where it is avoided), and keeps
+//                   maximum and sum in registers;
 //   warp 8          TMA: the two Q tiles once, K and V blocks into two-stage
 //                   rings;
 //   warp 9          MMA issuer: S_i = Q_i K^T (both from shared memory) and
@@ -25,9 +27,9 @@
 //
 // Measured (16/8 heads of 128, bf16): 8192 tokens, all visible, 0.25 ms (1080
 // TFLOP/s of visible work); 16384 tokens, window 2048 and 64 sinks, 0.28 ms (940).
-// In the first of these an iteration takes 4100 cycles where its 32 products need
-// 2048 (487000 cycles, 119 iterations in the busiest block, 112 in the average
-// one; tensor pipe 49%, issue slots 36%): the chain scores - softmax - product of
+// In the first of these an iteration takes 3900 cycles where its 32 products need
+// 2048 (469000 cycles, 119 iterations in the busiest block, 112 in the average
+// one; tensor pipe 50%, issue slots 37%): the chain scores - softmax - product of
 // one tile, of which the other tile's hides a half.  Neither fewer
 // special-function exponentials nor an earlier hand-over of half of P shortened it.
 #include <algorithm>
