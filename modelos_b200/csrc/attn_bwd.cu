@@ -890,11 +890,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         if (++q == w.nq) q = 0;
         uint32_t v[32];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) v[x] = pack2<T>(p[2 * x], p[2 * x + 1]);
+        for (int x = 0; x < 32; ++x)
+          v[x] = EXACT ? pack2_down<T>(p[2 * x], p[2 * x + 1]) : pack2<T>(p[2 * x], p[2 * x + 1]);
         tmem_st_32x32b_x32(ts, v);
         if constexpr (EXACT) {
+          uint32_t first;
 #pragma unroll
-          for (int x = 0; x < 32; ++x) v[x] = remainder2<T>(p[2 * x], p[2 * x + 1], v[x]);
+          for (int x = 0; x < 32; ++x) parts2<T>(p[2 * x], p[2 * x + 1], first, v[x]);
           tmem_st_32x32b_x32(ts + 32, v);
         }
         tmem_st_wait();

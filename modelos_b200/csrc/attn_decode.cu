@@ -395,13 +395,18 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
             const float p2 = ex2(x[sub][nt][2] - ma), p3 = ex2(x[sub][nt][3] - mb);
             l[nt][0] += p0 + p2;
             l[nt][1] += p1 + p3;
-            const uint32_t h0 = pack2<T>(p0, p1), h1 = pack2<T>(p2, p3);
-            pb[sub][nt][0] = transpose8x8(h0);
-            pb[sub][nt][1] = transpose8x8(h1);
-            if constexpr (!Q4) {
-              pl[sub][nt][0] = transpose8x8(remainder2<T>(p0, p1, h0));
-              pl[sub][nt][1] = transpose8x8(remainder2<T>(p2, p3, h1));
+            uint32_t h[2], r[2];
+            if constexpr (Q4) {
+              h[0] = pack2<T>(p0, p1);
+              h[1] = pack2<T>(p2, p3);
+            } else {
+              parts2<T>(p0, p1, h[0], r[0]);
+              parts2<T>(p2, p3, h[1], r[1]);
+              pl[sub][nt][0] = transpose8x8(r[0]);
+              pl[sub][nt][1] = transpose8x8(r[1]);
             }
+            pb[sub][nt][0] = transpose8x8(h[0]);
+            pb[sub][nt][1] = transpose8x8(h[1]);
           }
         }
         // ---- O^T += V^T P^T; keys behind the stage's count may hold anything
@@ -452,22 +457,27 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
             const uint32_t vb = buf + F::SIDE + kr * 128;
             const uint32_t keep0 = (2 * t < rest ? 0xffffu : 0u) | (2 * t + 1 < rest ? 0xffff0000u : 0u);
             const uint32_t keep1 = (2 * t + 8 < rest ? 0xffffu : 0u) | (2 * t + 9 < rest ? 0xffff0000u : 0u);
+            // (a tile's second product a step later, so as not to wait for its first)
+            uint32_t r[2][4];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              uint32_t r[4];
-              const int ch = (s & 3) * 2 + ((lane >> 3) & 1);
-              ldsm4t(r, vb + (s >> 2) * (F::KEYS * 128) + ((ch ^ (lane & 7)) << 4));
-              if (rest < 16) {
-                r[0] &= keep0;
-                r[1] &= keep0;
-                r[2] &= keep1;
-                r[3] &= keep1;
-              }
+            for (int s = 0; s <= KS; ++s) {
+              if (s < KS) {
+                uint32_t(&v)[4] = r[s & 1];
+                const int ch = (s & 3) * 2 + ((lane >> 3) & 1);
+                ldsm4t(v, vb + (s >> 2) * (F::KEYS * 128) + ((ch ^ (lane & 7)) << 4));
+                if (rest < 16) {
+                  v[0] &= keep0;
+                  v[1] &= keep0;
+                  v[2] &= keep1;
+                  v[3] &= keep1;
+                }
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816<T>(o[nt][s], r, pb[sub][nt][0], pb[sub][nt][1]);
-                mma16816<T>(o[nt][s], r, pl[sub][nt][0], pl[sub][nt][1]);
+                for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][s], v, pb[sub][nt][0], pb[sub][nt][1]);
               }
+              if (s > 0)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma16816<T>(o[nt][s - 1], r[(s - 1) & 1], pl[sub][nt][0], pl[sub][nt][1]);
             }
           }
         }

@@ -413,8 +413,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
             const float p1 = ex2(fmaf(__uint_as_float(s[x * 64 + 2 * y + 1]), c, -mm));
             l4[2 * (y & 1)] += p0;
             l4[2 * (y & 1) + 1] += p1;
-            p[y] = pack2<T>(p0, p1);
-            if constexpr (EXACT) lo[y] = remainder2<T>(p0, p1, p[y]);
+            if constexpr (EXACT)
+              parts2<T>(p0, p1, p[y], lo[y]);
+            else
+              p[y] = pack2<T>(p0, p1);
           }
           tmem_st_32x32b_x32(ts + x * 32, p);
           if constexpr (EXACT) tmem_st_32x32b_x32(ts + 64 + x * 32, lo);

@@ -145,6 +145,30 @@ __device__ __forceinline__ uint32_t remainder2(float x, float y, uint32_t w) {
   return pack2<T>(x - f[0], y - f[1]);
 }
 
+// Probabilities (not negative) as two packed parts for two products.  The first is
+// rounded towards 0, so that the second is not negative, and where the first is
+// not 0 the second is at least the type's smallest number: times an infinite value
+// both parts are that infinity, and their sum is not NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2_down(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2_down<__nv_bfloat16>(float x, float y) {
+  uint32_t w;
+  asm("cvt.rz.bf16x2.f32 %0, %2, %1;" : "=r"(w) : "f"(x), "f"(y));
+  return w;
+}
+template <>
+__device__ __forceinline__ uint32_t pack2_down<__half>(float x, float y) {
+  uint32_t w;
+  asm("cvt.rz.f16x2.f32 %0, %2, %1;" : "=r"(w) : "f"(x), "f"(y));
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void parts2(float x, float y, uint32_t& first, uint32_t& second) {
+  first = pack2_down<T>(x, y);
+  second = __vmaxu2(remainder2<T>(x, y, first), __vsetne2(first, 0u));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -155,3 +155,26 @@ def test_groups_of_the_4_bit_cache_that_read_back_as_nan(dtype, D, side):
                 got = got.clone()
                 got[1, :, :-1] = 0
             compare(got, want, tol, (side, Tq, window))
+
+
+@pytest.mark.parametrize("shape", SHAPES + [(2, 2, 1, 24, 24), (1, 40, 1, 100, 128)])
+@pytest.mark.parametrize("dtype,D", [(BF, 128), (HF, 64), (BF, 72)])
+def test_an_infinite_value(shape, dtype, D):
+    """inf in its channel for the rows that see it (also where probabilities take
+    part in two products), and in dv's channel for an infinite output gradient."""
+    from modelos_b200.attention import window_attention
+    B, Hq, Hk, Tq, Tk = shape
+    q, k, v, dout = make(B, Hq, Hk, Tq, Tk, D, dtype, seed=Tk)
+    key = 7 if Tk > Tq else 0  # all rows see it
+    v[0, 0, key, 3], v[-1, -1, key, 5] = INF, -INF
+    out = window_attention(q, k, v)
+    want = torch.zeros_like(out)
+    G = Hq // Hk
+    want[0, :G, :, 3], want[-1, -G:, :, 5] = INF, -INF
+    assert torch.equal(out.isinf(), want.isinf()) and not out.isnan().any()
+    assert torch.equal(out[want.isinf()], want[want.isinf()])
+    # the last query sees all keys
+    leaves = [t.detach().requires_grad_() for t in make(B, Hq, Hk, Tq, Tk, D, dtype, seed=Tk)[:3]]
+    dout[0, 0, -1, 3] = INF
+    _, _, dv = torch.autograd.grad(window_attention(*leaves), leaves, dout)
+    assert (dv[0, 0, :, 3] == INF).all() and torch.isfinite(dv[0, 0, :, :3]).all()

@@ -16,8 +16,10 @@ BF, HF = torch.bfloat16, torch.float16
 
 def bounds(q, k, v, dout, window, sinks, scale, starts, ends):
     """Results in 64 bits and bounds on the kernels' error: what is held in the
-    operands' type is held with its remainder, u * u of it; scores, sums and
-    statistics are in 32 bits, the exponential is good to 2^-22."""
+    operands' type is held with its remainder, good to u * u of it (probabilities
+    2 u * u: their first part is rounded down, and a remainder of 0 is held as the
+    type's smallest number, 2 ``least``); scores, sums and statistics are in 32 bits,
+    the exponential is good to 2^-22."""
     u, f32 = torch.finfo(q.dtype).eps / 2, attnref.F32
     least = torch.finfo(q.dtype).smallest_normal * u
     B, Hq, Tq, D = q.shape
@@ -30,8 +32,8 @@ def bounds(q, k, v, dout, window, sinks, scale, starts, ends):
     seen = see.double().expand_as(p)
     size = (q.abs() @ ks.abs().transpose(-1, -2)) * abs(scale)
     n, m = see.sum(-1).amax().item(), Tq * (Hq // Hk)
-    one = 1.01 * u * u + 2 * (2.0 ** -20 + (D + 8) * f32 * (size * see).amax().item()) + (n + 16) * f32
-    ep = p * one + least * seen
+    one = 2.02 * u * u + 2 * (2.0 ** -20 + (D + 8) * f32 * (size * see).amax().item()) + (n + 16) * f32
+    ep = p * one + 2 * least * seen
     r = dict(out=(out, u * out.abs() * (1 + u) + ep @ vs.abs()))
     dp = do @ vs.transpose(-1, -2)
     delta = (p * dp).sum(-1, keepdim=True)
