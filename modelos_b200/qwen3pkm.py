@@ -125,7 +125,7 @@ def _attention_mask(batch_size, q_length, kv_length, q_offset=0, kv_offset=0, ma
         raise ValueError(f"modelos_b200 attention: the mask has {attention_mask.shape[1]} columns for "
                          f"{kv_offset + kv_length} tokens")
     bounds = attention_bounds(attention_mask, kv_length, kv_offset)
-    # where all queries are padding, nothing is visible: KVCache4.attend takes no ends
+    # where all queries are padding, nothing is visible (KVCache4.attend takes no ends)
     bounds[0].masked_fill_(bounds[1] <= kv_length - q_length, kv_length)
     return bounds
 
@@ -152,6 +152,9 @@ def _attention(module, query, key, value, attention_mask, scaling=None, dropout=
     starts, ends = (None, None) if attention_mask is None else attention_mask.unbind()
     if isinstance(key, KVCache4):
         out = key.attend(query, window=sliding_window, sinks=sinks, scale=scaling, starts=starts)
+        if ends is not None and query.shape[2] > 1:  # (a token alone: its starts say so)
+            at = key.lengths[:, None] - query.shape[2] + torch.arange(query.shape[2], device=query.device)
+            out = out.masked_fill((at >= ends[:, None])[:, None, :, None], 0)
     else:
         out = window_attention(query, key, value, window=sliding_window, sinks=sinks, scale=scaling, starts=starts,
                                ends=ends)

@@ -185,3 +185,20 @@ def test_rows_whose_tokens_are_all_padding_over_the_4_bit_cache(kw):
                 steps.append(out.logits[1:])
             logits.append(torch.cat(steps, 1))
     assert torch.equal(*logits)  # (the attention's output is 0 in every layer)
+
+
+def test_padding_behind_a_few_tokens_over_the_4_bit_cache():
+    """Some of a few tokens are padding: they see nothing, as over the 16-bit cache,
+    so that their logits come from themselves alone."""
+    m = model(WINDOW)
+    x, mask = ids(3, 12), torch.ones(3, 12, dtype=torch.long)
+    mask[1, 10:] = 0
+    mask[2, 11:] = 0
+    logits = []
+    with torch.no_grad():
+        for cache in (None, qwen3pkm.QuantizedCache(m.config, 16)):
+            out = m(x[:, :8], attention_mask=mask[:, :8], past_key_values=cache, use_cache=True)
+            logits.append(m(x[:, 8:], attention_mask=mask, past_key_values=out.past_key_values).logits)
+    padding = ~mask[:, 8:].bool()
+    assert torch.equal(logits[0][padding], logits[1][padding])
+    assert rel(logits[1], logits[0]) < 0.16  # 4 bits in two layers: 0.08 * 4 ** 0.5
