@@ -16,8 +16,8 @@
 // goes to the copies.  The running maximum of a row is raised only when a
 // score exceeds it by more than 2^8 (which a vote finds without reducing).
 //
-// Measured (16/8 heads of 128, bf16): 32 sequences with 8196 visible keys, 156 us
-// (6.9 TB/s, at the memory's rate); 8 with 2305, 12 us (6.2 TB/s).  4 bits, 32
+// Measured (16/8 heads of 128, bf16): 32 sequences with 8196 visible keys, 157 us
+// (6.8 TB/s, at the memory's rate); 8 with 2305, 12.8 us (5.9 TB/s).  4 bits, 32
 // sequences of 14100 to 16000 keys: 169 us (3.6 TB/s), bound by instructions: 428
 // for 16 keys, 240 of them make codes into values.
 //
@@ -381,10 +381,10 @@ __global__ void __launch_bounds__(DecodeTile<DP, NT, Q4>::THREADS, DecodeTile<DP
           }
         }
         // Probabilities in the keys' type for the product.  16 bits: with what
-        // their rounding left as a second product, which the time, the copies',
-        // does not show; without it the output's error was 1.4 times that of its
-        // own rounding.  4 bits: the kernel is bound by instructions, and the
-        // codes' error is many times larger.
+        // their rounding left as a second product, without which the output's error
+        // was 1.3 times that of its own rounding; the copies are what bounds the
+        // kernel (8196 keys, 32 sequences: 156 -> 157 us; 2305 keys, 8: 12.2 -> 12.8).
+        // 4 bits: bound by instructions, and the codes' error is many times larger.
         uint32_t pb[F::SUB][NT][2], pl[F::SUB][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
